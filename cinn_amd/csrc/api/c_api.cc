@@ -189,6 +189,24 @@ const std::map<std::string, Method>& Methods() {
       return b.BatchNormGrad(in.at(0), in.at(1), in.at(2), in.at(3), in.at(4), GetAttr<float>(a, "epsilon", 1e-5f),
                              GetAttr<std::string>(a, "data_layout", "NCHW"));
     };
+    auto rotary_options = [](const AttributeMap& a) {
+      NetBuilder::RotaryOptions o;
+      o.rotary_dim      = GetAttr<int>(a, "rotary_dim", o.rotary_dim);
+      o.interleaved     = GetAttr<bool>(a, "interleaved", o.interleaved);
+      o.theta           = GetAttr<double>(a, "theta", o.theta);
+      o.factor          = GetAttr<double>(a, "factor", o.factor);
+      o.original_length = GetAttr<int>(a, "original_length", o.original_length);
+      o.low             = GetAttr<double>(a, "low", o.low);
+      o.high            = GetAttr<double>(a, "high", o.high);
+      o.magnitude       = GetAttr<double>(a, "magnitude", o.magnitude);
+      return o;
+    };
+    m["RotaryEmbedding"] = [=](NetBuilder& b, const std::vector<Variable>& in, const AttributeMap& a) {
+      return std::vector<Variable>{b.RotaryEmbedding(in.at(0), in.at(1), GetAttr<int>(a, "heads", 0), rotary_options(a))};
+    };
+    m["RotaryEmbeddingGrad"] = [=](NetBuilder& b, const std::vector<Variable>& in, const AttributeMap& a) {
+      return std::vector<Variable>{b.RotaryEmbeddingGrad(in.at(0), in.at(1), GetAttr<int>(a, "heads", 0), rotary_options(a))};
+    };
     m["Pool2d"] = [](NetBuilder& b, const std::vector<Variable>& in, const AttributeMap& a) {
       return std::vector<Variable>{
           b.Pool2d(in.at(0), GetAttr<std::string>(a, "pooling_type", "max"), GetAttr<std::vector<int>>(a, "ksize", {1, 1}),

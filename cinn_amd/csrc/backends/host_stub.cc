@@ -19,6 +19,7 @@ namespace {
 
 int I(const BakedArg& a) { return static_cast<int>(a.i); }
 float F(const BakedArg& a) { return static_cast<float>(a.f); }
+double D(const BakedArg& a) { return a.f; }
 bool B(const BakedArg& a) { return a.i != 0; }
 
 // Argument lists below follow the call the lowering builds: (kernel_args, kernel_args_num, <constants...>,
@@ -86,6 +87,10 @@ void InvokeChannelGradient(const std::vector<BakedArg>& a, void* args, int32_t n
 void InvokeAttention(const std::vector<BakedArg>& a, void* args, int32_t n, void* stream) {
   cinn_call_hip_attention(args, n, F(a[2]), I(a[3]), I(a[4]), I(a[5]), I(a[6]), I(a[7]), I(a[8]), I(a[9]), I(a[10]), I(a[11]), stream);
 }
+void InvokeRotaryEmbedding(const std::vector<BakedArg>& a, void* args, int32_t n, void* stream) {
+  cinn_call_hip_rotary_embedding(args, n, I(a[2]), I(a[3]), I(a[4]), I(a[5]), I(a[6]), I(a[7]), I(a[8]), D(a[9]), D(a[10]), I(a[11]),
+                                 D(a[12]), D(a[13]), D(a[14]), stream);
+}
 void InvokeBatchedCublas(const std::vector<BakedArg>& a, void* args, int32_t n, void* stream) {
   cinn_call_batched_cublas(args, n, I(a[2]), B(a[3]), B(a[4]), B(a[5]), F(a[6]), F(a[7]), I(a[8]), I(a[9]), I(a[10]),
                            I(a[11]), I(a[12]), I(a[13]), I(a[14]), I(a[15]), stream);
@@ -135,6 +140,9 @@ ExternApiRegistry::ExternApiRegistry() {
   Register("cinn_call_hip_top_k", InvokeTopK, 9);
   // (kernel_args, kernel_args_num, scale, batch, heads, queries, keys, appended, d, operands, layouts, parts, kernel_stream)
   Register("cinn_call_hip_attention", InvokeAttention, 13);
+  // (kernel_args, kernel_args_num, tokens, heads, total_heads, d, rotary_dim, interleaved, transposed, theta, factor,
+  // original_length, low, high, magnitude, kernel_stream)
+  Register("cinn_call_hip_rotary_embedding", InvokeRotaryEmbedding, 16);
   // (kernel_args, kernel_args_num, trans_b, m, n, k, kernel_stream)
   Register("cinn_call_hip_matmul_bias", InvokeMatmulBias, 7);
   // (kernel_args, kernel_args_num, m, n, k, operands, outputs, epsilon, gelu, kernel_stream)

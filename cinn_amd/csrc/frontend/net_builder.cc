@@ -319,6 +319,27 @@ std::vector<Variable> NetBuilder::BatchNormGrad(const Variable& dy, const Variab
 }
 
 namespace {
+utils::AttributeMap RotaryAttrs(int heads, const NetBuilder::RotaryOptions& o, bool transposed) {
+  return {{"heads", heads},
+          {"rotary_dim", o.rotary_dim},
+          {"interleaved", o.interleaved},
+          {"transposed", transposed},
+          {"theta", o.theta},
+          {"factor", o.factor},
+          {"original_length", o.original_length},
+          {"low", o.low},
+          {"high", o.high},
+          {"magnitude", o.magnitude}};
+}
+}  // namespace
+Variable NetBuilder::RotaryEmbedding(const Variable& x, const Variable& positions, int heads, const RotaryOptions& options) {
+  return CustomInstr("rotary_embedding", {x, positions}, RotaryAttrs(heads, options, false)).front();
+}
+Variable NetBuilder::RotaryEmbeddingGrad(const Variable& dy, const Variable& positions, int heads, const RotaryOptions& options) {
+  return CustomInstr("rotary_embedding", {dy, positions}, RotaryAttrs(heads, options, true)).front();
+}
+
+namespace {
 utils::AttributeMap Pool2dAttrs(const Variable& x, const std::string& pooling_type, const std::vector<int>& ksize,
                          const std::vector<int>& strides, const std::vector<int>& paddings, bool ceil_mode,
                          bool exclusive, bool global_pooling, const std::string& data_format, bool adaptive,

@@ -114,6 +114,18 @@ class NetBuilder {
   std::vector<Variable> BatchNormGrad(const Variable& dy, const Variable& x, const Variable& scale,
                                       const Variable& save_mean, const Variable& save_variance, float epsilon = 1e-5f,
                                       const std::string& data_layout = "NCHW");
+  // Rotary positions of the first `heads` heads (0: all) of x [..., heads, d] at positions [...], rotary_dim elements of each
+  // (0: all), and x's gradient from dy of y's shape; theta, scaling and the order of pairs as in
+  // cinn_call_hip_rotary_embedding.  No counterpart in the reference.
+  struct RotaryOptions {
+    int rotary_dim{0};
+    bool interleaved{false};
+    double theta{10000.0}, factor{1.0};
+    int original_length{0};
+    double low{1.0}, high{4.0}, magnitude{1.0};
+  };
+  Variable RotaryEmbedding(const Variable& x, const Variable& positions, int heads, const RotaryOptions& options);
+  Variable RotaryEmbeddingGrad(const Variable& dy, const Variable& positions, int heads, const RotaryOptions& options);
   Variable Pool2d(const Variable& x, const std::string& pooling_type, const std::vector<int>& ksize,
                   const std::vector<int>& strides = {1, 1}, const std::vector<int>& paddings = {0, 0},
                   bool ceil_mode = false, bool exclusive = true, bool global_pooling = false,

@@ -1623,6 +1623,22 @@ ir::LoweredFuncRef OpLowerer::LowerLibraryCall(const Group& group) const {
       operands |= static_cast<int>(std::find(group.inputs.begin(), group.inputs.end(), in) - group.inputs.begin()) << (4 * s);
     }
     push_ints({operands, GetAttr<int>(n->attrs, "layouts", 0), GetAttr<int>(n->attrs, "parts", 1)});
+  } else if (op == "rotary_embedding") {
+    api           = "cinn_call_hip_rotary_embedding";
+    const auto& x = n->inputs[0]->shape;
+    const auto& y = n->outputs[0]->shape;
+    const int d = x.back(), total_heads = x[x.size() - 2], rotary_dim = GetAttr<int>(n->attrs, "rotary_dim", 0);
+    push_ints({static_cast<int>(ShapeNumel(x) / d / total_heads), y[y.size() - 2], total_heads, d, rotary_dim > 0 ? rotary_dim : d});
+    push_ints({GetAttr<bool>(n->attrs, "interleaved", false) ? 1 : 0, GetAttr<bool>(n->attrs, "transposed", false) ? 1 : 0});
+    auto push_double = [&](const char* name, double dflt) {
+      args.push_back(ir::MakeFloatImm(common::Float(64), GetAttr<double>(n->attrs, name, dflt)));
+    };
+    push_double("theta", 10000.0);
+    push_double("factor", 1.0);
+    push_ints({GetAttr<int>(n->attrs, "original_length", 0)});
+    push_double("low", 1.0);
+    push_double("high", 4.0);
+    push_double("magnitude", 1.0);
   } else {
     CINN_CHECK(false) << "op " << op << " has no GPU lowering";
   }

@@ -794,6 +794,38 @@ OpRegistry::OpRegistry() {
     op.infer_dtype = SameTypeAsFirst;
   }
   {
+    // x [..., total heads, d], positions [...] -> the first `heads` heads (0: all), turned by their positions; transposed: the
+    // gradient
+    auto& op       = r->Register("rotary_embedding");
+    op.pattern     = OpPatternKind::kNonFusible;
+    op.num_inputs  = 2;
+    op.infer_shape = [](const std::vector<ShapeType>& in, const AttributeMap& a) {
+      CINN_CHECK_GE(in[0].size(), 2u) << "rotary_embedding: x is [..., heads, d]";
+      const int d = in[0].back(), total = in[0][in[0].size() - 2];
+      CINN_CHECK(in[1] == ShapeType(in[0].begin(), in[0].end() - 2) || (in[0].size() == 2 && in[1] == ShapeType{1}))
+          << "rotary_embedding: one position for each [heads, d] of x is expected";
+      const int heads = GetAttr<int>(a, "heads", 0), rotary_dim = GetAttr<int>(a, "rotary_dim", 0);
+      CINN_CHECK(heads >= 0 && heads <= total) << "rotary_embedding: " << heads << " of " << total << " heads";
+      const int r = rotary_dim == 0 ? d : rotary_dim;
+      CINN_CHECK(r > 0 && r % 2 == 0 && r <= d && r <= 512)
+          << "rotary_embedding: rotary_dim " << r << " of " << d << " elements: an even number of at most 512 is wanted";
+      const double theta = GetAttr<double>(a, "theta", 10000.0), factor = GetAttr<double>(a, "factor", 1.0);
+      CINN_CHECK(std::isfinite(theta) && theta > 0 && std::isfinite(factor) && factor > 0) << "rotary_embedding: theta and factor are positive";
+      const int original = GetAttr<int>(a, "original_length", 0);
+      const double low = GetAttr<double>(a, "low", 1.0), high = GetAttr<double>(a, "high", 4.0);
+      CINN_CHECK(original >= 0 && (original == 0 || (std::isfinite(low) && std::isfinite(high) && high > low)))
+          << "rotary_embedding: original_length " << original << ", low " << low << ", high " << high;
+      ShapeType out        = in[0];
+      out[out.size() - 2] = heads == 0 ? total : heads;
+      return std::vector<ShapeType>{out};
+    };
+    op.infer_dtype = [](const std::vector<Type>& in, const AttributeMap&) {
+      CINN_CHECK(in[0].is_float(32) || in[0].is_float(16) || in[0].is_bfloat16()) << "rotary_embedding: x is fp16, bf16 or fp32";
+      CINN_CHECK(in[1].is_int(32) || in[1].is_int(64)) << "rotary_embedding: positions are int32 or int64";
+      return std::vector<Type>{in[0]};
+    };
+  }
+  {
     // pooling output size and attribute meaning as cinn/hlir/pe/nn.cc:956-1109 (PoolImpl)
     auto& op       = r->Register("pool2d");
     op.pattern     = OpPatternKind::kNonFusible;

@@ -65,6 +65,8 @@ def _attr_string(attrs):
             items.append("%s:b=%d" % (key, int(value)))
         elif isinstance(value, (int, np.integer)):
             items.append("%s:i=%d" % (key, int(value)))
+        elif isinstance(value, ctypes.c_double):
+            items.append("%s:d=%r" % (key, value.value))
         elif isinstance(value, (float, np.floating)):
             items.append("%s:f=%r" % (key, float(value)))
         elif isinstance(value, str):
@@ -249,6 +251,29 @@ class NetBuilder(object):
                            strides=list(stride), paddings=list(padding), ceil_mode=ceil_mode, exclusive=exclusive,
                            global_pooling=global_pooling, data_format=data_format, adaptive=adaptive,
                            padding_algorithm=padding_algorithm)
+
+    def _rotary(self, method, x, positions, heads, rotary_dim, interleaved, theta, factor, original_length, low, high, magnitude):
+        wide = dict(theta=theta, factor=factor, low=low, high=high, magnitude=magnitude)
+        return self._call1(method, [x, positions], heads=int(heads), rotary_dim=int(rotary_dim), interleaved=bool(interleaved),
+                           original_length=int(original_length), **{k: ctypes.c_double(v) for k, v in wide.items()})
+
+    def rotary_embedding(self, x, positions, heads=0, rotary_dim=0, interleaved=False, theta=10000.0, factor=1.0,
+                         original_length=0, low=1.0, high=4.0, magnitude=1.0):
+        """Rotary positions of the first `heads` heads (0: all) of x [..., heads, d] at `positions` [...] (int32 or int64);
+        the result holds those heads only.
+
+        Pair i < rotary_dim / 2 of a head - elements i and i + rotary_dim / 2, or 2 i and 2 i + 1 if `interleaved` - is
+        turned by position * f_i and multiplied by `magnitude`; elements from rotary_dim (0: d) on are copied.  f_i =
+        theta ** (-2 i / rotary_dim), divided by `factor`; with an original_length only frequencies of fewer than `high`
+        turns within it are: those under `low` turns wholly, those between in proportion."""
+        return self._rotary("RotaryEmbedding", x, positions, heads, rotary_dim, interleaved, theta, factor, original_length,
+                            low, high, magnitude)
+
+    def rotary_embedding_grad(self, dy, positions, heads=0, rotary_dim=0, interleaved=False, theta=10000.0, factor=1.0,
+                              original_length=0, low=1.0, high=4.0, magnitude=1.0):
+        """Gradient of the heads that rotary_embedding turned, from that of its result: the same arguments with dy for x."""
+        return self._rotary("RotaryEmbeddingGrad", dy, positions, heads, rotary_dim, interleaved, theta, factor,
+                            original_length, low, high, magnitude)
 
     def paddle_layer_norm(self, x, scale=None, bias=None, epsilon=1e-5, begin_norm_axis=1):
         """layer_norm as the Paddle op mapper composes it; returns [y, mean, variance]."""

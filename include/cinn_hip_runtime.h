@@ -281,6 +281,17 @@ void cinn_call_hip_top_k(void* v_args, int num_args, int outer, int size, int in
 void cinn_call_hip_attention(void* v_args, int num_args, float scale, int batch, int heads, int queries, int keys,
                              int appended, int d, int operands, int layouts, int parts, void* stream);
 
+/* Rotary positions: y [tokens][heads][d] from the first `heads` heads of x [tokens][total_heads][d]; fp16 / bf16 / fp32, positions
+ * [tokens] int32 or int64.  Pair i < rotary_dim / 2 of a head, its elements 2 i and 2 i + 1 (interleaved) or i and
+ * i + rotary_dim / 2, is turned by position * f_i and multiplied by magnitude, f_i = theta^(-2 i / rotary_dim) scaled:
+ * divided by factor, or with original_length > 0 multiplied by g + (1 - g) / factor, g = (original_length f_i / 2 pi - low) /
+ * (high - low) between 0 and 1.  Elements from rotary_dim (even, at most 512) on are copied.  transposed: the transpose of
+ * that, which makes x's gradient of y's.  Angles in 64 bits, products in fp32, one rounding.  v_args = {x, positions, y}; y
+ * does not overlap x.  No counterpart in the reference. */
+void cinn_call_hip_rotary_embedding(void* v_args, int num_args, int tokens, int heads, int total_heads, int d, int rotary_dim,
+                                    int interleaved, int transposed, double theta, double factor, int original_length,
+                                    double low, double high, double magnitude, void* stream);
+
 /* C [m][n] = A [m][k] op(B) + bias, one rounding; B is [k][n], or [n][k] with trans_b.  fp16 / bf16 / fp32 with a bias [n]
  * of the same type or fp32; n and k below 2^22.  v_args = {A, B, bias, C}, or {A, bias, C} where B is A. */
 void cinn_call_hip_matmul_bias(void* v_args, int num_args, int trans_b, int m, int n, int k, void* stream);
