@@ -189,6 +189,19 @@ const std::map<std::string, Method>& Methods() {
       return b.BatchNormGrad(in.at(0), in.at(1), in.at(2), in.at(3), in.at(4), GetAttr<float>(a, "epsilon", 1e-5f),
                              GetAttr<std::string>(a, "data_layout", "NCHW"));
     };
+    auto attention_options = [](const AttributeMap& a) {
+      NetBuilder::AttentionOptions o;
+      o.scale    = GetAttr<float>(a, "scale", o.scale);
+      o.heads    = GetAttr<int>(a, "heads", o.heads);
+      o.kv_heads = GetAttr<int>(a, "kv_heads", o.kv_heads);
+      o.q_head   = GetAttr<int>(a, "q_head", o.q_head);
+      o.k_head   = GetAttr<int>(a, "k_head", o.k_head);
+      o.v_head   = GetAttr<int>(a, "v_head", o.v_head);
+      return o;
+    };
+    m["PackedAttention"] = [=](NetBuilder& b, const std::vector<Variable>& in, const AttributeMap& a) {
+      return std::vector<Variable>{b.PackedAttention(in.at(0), in.at(1), in.at(2), in.at(3), attention_options(a))};
+    };
     auto rotary_options = [](const AttributeMap& a) {
       NetBuilder::RotaryOptions o;
       o.rotary_dim      = GetAttr<int>(a, "rotary_dim", o.rotary_dim);

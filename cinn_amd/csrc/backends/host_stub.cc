@@ -87,6 +87,10 @@ void InvokeChannelGradient(const std::vector<BakedArg>& a, void* args, int32_t n
 void InvokeAttention(const std::vector<BakedArg>& a, void* args, int32_t n, void* stream) {
   cinn_call_hip_attention(args, n, F(a[2]), I(a[3]), I(a[4]), I(a[5]), I(a[6]), I(a[7]), I(a[8]), I(a[9]), I(a[10]), I(a[11]), stream);
 }
+void InvokePackedAttention(const std::vector<BakedArg>& a, void* args, int32_t n, void* stream) {
+  cinn_call_hip_packed_attention(args, n, F(a[2]), I(a[3]), I(a[4]), I(a[5]), I(a[6]), I(a[7]), I(a[8]), I(a[9]), I(a[10]), I(a[11]),
+                                 I(a[12]), I(a[13]), I(a[14]), stream);
+}
 void InvokeRotaryEmbedding(const std::vector<BakedArg>& a, void* args, int32_t n, void* stream) {
   cinn_call_hip_rotary_embedding(args, n, I(a[2]), I(a[3]), I(a[4]), I(a[5]), I(a[6]), I(a[7]), I(a[8]), D(a[9]), D(a[10]), I(a[11]),
                                  D(a[12]), D(a[13]), D(a[14]), stream);
@@ -140,6 +144,9 @@ ExternApiRegistry::ExternApiRegistry() {
   Register("cinn_call_hip_top_k", InvokeTopK, 9);
   // (kernel_args, kernel_args_num, scale, batch, heads, queries, keys, appended, d, operands, layouts, parts, kernel_stream)
   Register("cinn_call_hip_attention", InvokeAttention, 13);
+  // (kernel_args, kernel_args_num, scale, tokens, sequences, heads, kv_heads, d, operands, heads of q and the first in use, of
+  // k, of v, kernel_stream)
+  Register("cinn_call_hip_packed_attention", InvokePackedAttention, 16);
   // (kernel_args, kernel_args_num, tokens, heads, total_heads, d, rotary_dim, interleaved, transposed, theta, factor,
   // original_length, low, high, magnitude, kernel_stream)
   Register("cinn_call_hip_rotary_embedding", InvokeRotaryEmbedding, 16);

@@ -319,6 +319,16 @@ std::vector<Variable> NetBuilder::BatchNormGrad(const Variable& dy, const Variab
 }
 
 namespace {
+utils::AttributeMap AttentionAttrs(const NetBuilder::AttentionOptions& o) {
+  return {{"scale", o.scale}, {"heads", o.heads}, {"kv_heads", o.kv_heads}, {"q_head", o.q_head}, {"k_head", o.k_head}, {"v_head", o.v_head}};
+}
+}  // namespace
+Variable NetBuilder::PackedAttention(const Variable& q, const Variable& k, const Variable& v, const Variable& offsets,
+                                     const AttentionOptions& options) {
+  return CustomInstr("packed_attention", {q, k, v, offsets}, AttentionAttrs(options)).front();
+}
+
+namespace {
 utils::AttributeMap RotaryAttrs(int heads, const NetBuilder::RotaryOptions& o, bool transposed) {
   return {{"heads", heads},
           {"rotary_dim", o.rotary_dim},

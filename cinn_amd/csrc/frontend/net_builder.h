@@ -114,6 +114,15 @@ class NetBuilder {
   std::vector<Variable> BatchNormGrad(const Variable& dy, const Variable& x, const Variable& scale,
                                       const Variable& save_mean, const Variable& save_variance, float epsilon = 1e-5f,
                                       const std::string& data_layout = "NCHW");
+  // Attention with grouped heads, scaled by `scale`: `heads` query heads from q_head on in q's tensor share `kv_heads` from
+  // k_head and v_head on in k's and v's (0 heads: all from there on), so that q, k and v may be one tensor of packed
+  // projections.  No counterpart in the reference.
+  struct AttentionOptions {
+    float scale{1.0f};
+    int heads{0}, kv_heads{0}, q_head{0}, k_head{0}, v_head{0};
+  };
+  // causal, over sequences packed behind one another in [tokens, heads, d] (cinn_call_hip_packed_attention)
+  Variable PackedAttention(const Variable& q, const Variable& k, const Variable& v, const Variable& offsets, const AttentionOptions& options);
   // Rotary positions of the first `heads` heads (0: all) of x [..., heads, d] at positions [...], rotary_dim elements of each
   // (0: all), and x's gradient from dy of y's shape; theta, scaling and the order of pairs as in
   // cinn_call_hip_rotary_embedding.  No counterpart in the reference.

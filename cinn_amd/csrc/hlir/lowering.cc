@@ -1375,6 +1375,26 @@ ir::LoweredFuncRef OpLowerer::LowerLibraryCall(const Group& group) const {
   auto push_ints = [&](std::initializer_list<int> vals) {
     for (int v : vals) args.push_back(I32(v));
   };
+  // four bits per input: which of the call's arguments it is (equal values are one)
+  auto operand_slots = [&] {
+    uint32_t slots = 0;
+    for (size_t s = 0; s < n->inputs.size(); ++s)
+      slots |= static_cast<uint32_t>(std::find(group.inputs.begin(), group.inputs.end(), n->inputs[s]) - group.inputs.begin()) << (4 * s);
+    return static_cast<int>(slots);
+  };
+  // rows of an attention are moved 16 bytes at a time
+  auto check_rows = [&] {
+    const NodeData* q = n->inputs[0];
+    CINN_CHECK_EQ(q->shape.back() * q->dtype.bytes() % 16, 0) << op << ": heads of " << q->shape.back() << " elements are no whole number of 16-byte chunks";
+  };
+  // q, k and v: how many heads the tensor has and the first one in use
+  auto push_attention_heads = [&] {
+    const char* first[] = {"q_head", "k_head", "v_head"};
+    for (int i = 0; i < 3; ++i) {
+      const auto& shape = n->inputs[i]->shape;
+      push_ints({shape[shape.size() - 2], GetAttr<int>(n->attrs, first[i], 0)});
+    }
+  };
   if (op == "matmul" || op == "mul") {
     // argument list of CustomCallArgsForCublas (cinn/hlir/op/custom_call.cc:116-217)
     api = "cinn_call_cublas";
@@ -1623,6 +1643,14 @@ ir::LoweredFuncRef OpLowerer::LowerLibraryCall(const Group& group) const {
       operands |= static_cast<int>(std::find(group.inputs.begin(), group.inputs.end(), in) - group.inputs.begin()) << (4 * s);
     }
     push_ints({operands, GetAttr<int>(n->attrs, "layouts", 0), GetAttr<int>(n->attrs, "parts", 1)});
+  } else if (op == "packed_attention") {
+    api            = "cinn_call_hip_packed_attention";
+    const auto& q  = n->inputs[0]->shape;
+    const int all  = n->outputs[0]->shape[1];
+    check_rows();
+    args.push_back(Expr(GetAttr<float>(n->attrs, "scale", 1.0f)));
+    push_ints({q[0], n->inputs[3]->shape[0] - 1, all, AttentionKvHeads(n->inputs[1]->shape[1], n->attrs), q[2], operand_slots()});
+    push_attention_heads();
   } else if (op == "rotary_embedding") {
     api           = "cinn_call_hip_rotary_embedding";
     const auto& x = n->inputs[0]->shape;

@@ -76,6 +76,9 @@ std::string ExternFuncName(const std::string& fn, const common::Type& type);
 
 int64_t ShapeNumel(const ShapeType& s);
 
+// key heads of an attention whose tensor of keys has `total` of them: the attribute kv_heads, or all from k_head on
+int AttentionKvHeads(int total, const AttributeMap& attrs);
+
 }  // namespace framework
 }  // namespace hlir
 }  // namespace cinn

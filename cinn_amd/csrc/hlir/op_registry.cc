@@ -21,6 +21,11 @@ std::string ExternFuncName(const std::string& fn, const Type& type) {
   return "cinn_hip_" + fn + "_" + common::TypeSuffix(type);
 }
 
+int AttentionKvHeads(int total, const AttributeMap& attrs) {
+  const int given = GetAttr<int>(attrs, "kv_heads", 0);
+  return given == 0 ? total - GetAttr<int>(attrs, "k_head", 0) : given;
+}
+
 OpRegistry& OpRegistry::Global() {
   static OpRegistry r;
   return r;
@@ -48,6 +53,36 @@ std::vector<std::string> OpRegistry::ListAllNames() const {
 }
 
 namespace {
+
+// q, k and v of an attention, [..., heads, d] each, of which `heads` from q_head, `kv_heads` from k_head and v_head on are in
+// use (0: all from there on): the shape of the result
+ShapeType AttentionShape(const char* op, const std::vector<ShapeType>& in, const AttributeMap& a, size_t rank) {
+  CINN_CHECK_GE(in.size(), 3u) << op << ": q, k and v are expected";
+  for (int i = 0; i < 3; ++i) {
+    CINN_CHECK_EQ(in[i].size(), rank) << op << ": operand " << i << " has the wrong rank";
+    CINN_CHECK(std::equal(in[0].begin(), in[0].end() - 2, in[i].begin()) && in[i].back() == in[0].back())
+        << op << ": q, k and v differ in more than their heads";
+  }
+  const int q_head = GetAttr<int>(a, "q_head", 0), k_head = GetAttr<int>(a, "k_head", 0), v_head = GetAttr<int>(a, "v_head", 0);
+  const int total = in[0][rank - 2], given = GetAttr<int>(a, "heads", 0);
+  const int heads = given == 0 ? total - q_head : given, kv_heads = AttentionKvHeads(in[1][rank - 2], a);
+  CINN_CHECK(q_head >= 0 && k_head >= 0 && v_head >= 0 && heads > 0 && kv_heads > 0 && q_head + heads <= total &&
+             k_head + kv_heads <= in[1][rank - 2] && v_head + kv_heads <= in[2][rank - 2])
+      << op << ": " << heads << " heads from " << q_head << " of " << total << ", " << kv_heads << " key heads from " << k_head << " of "
+      << in[1][rank - 2] << ", values from " << v_head << " of " << in[2][rank - 2];
+  CINN_CHECK_EQ(heads % kv_heads, 0) << op << ": " << heads << " heads do not share " << kv_heads << " key heads evenly";
+  CINN_CHECK(in[0].back() <= 128) << op << ": heads of at most 128 elements are supported, not " << in[0].back();
+  CINN_CHECK(std::isfinite(GetAttr<float>(a, "scale", 1.0f))) << op << ": scale";
+  ShapeType out = in[0];
+  out[rank - 2] = heads;
+  return out;
+}
+Type AttentionType(const char* op, const std::vector<Type>& in, size_t floating) {
+  CINN_CHECK(in[0].is_float(32) || in[0].is_float(16) || in[0].is_bfloat16()) << op << ": fp16, bf16 or fp32 is expected";
+  for (size_t i = 0; i < in.size(); ++i)
+    CINN_CHECK(i < floating ? in[i] == in[0] : in[i].is_int(32)) << op << ": operand " << i << (i < floating ? " differs in type from q" : " is not int32");
+  return in[0];
+}
 
 std::vector<ShapeType> SameShapeAsFirst(const std::vector<ShapeType>& in, const AttributeMap&) { return {in[0]}; }
 std::vector<Type> SameTypeAsFirst(const std::vector<Type>& in, const AttributeMap&) { return {in[0]}; }
@@ -792,6 +827,17 @@ OpRegistry::OpRegistry() {
       return std::vector<ShapeType>{GetAttr<std::vector<int>>(a, "out_shape", {})};
     };
     op.infer_dtype = SameTypeAsFirst;
+  }
+  {
+    // q, k, v [tokens, heads, d] and the offsets of the sequences in them
+    auto& op       = r->Register("packed_attention");
+    op.pattern     = OpPatternKind::kNonFusible;
+    op.num_inputs  = 4;
+    op.infer_shape = [](const std::vector<ShapeType>& in, const AttributeMap& a) {
+      CINN_CHECK(in[3].size() == 1 && in[3][0] >= 2) << "packed_attention: offsets hold the start of every sequence and the end of the last";
+      return std::vector<ShapeType>{AttentionShape("packed_attention", in, a, 3)};
+    };
+    op.infer_dtype = [](const std::vector<Type>& in, const AttributeMap&) { return std::vector<Type>{AttentionType("packed_attention", in, 3)}; };
   }
   {
     // x [..., total heads, d], positions [...] -> the first `heads` heads (0: all), turned by their positions; transposed: the

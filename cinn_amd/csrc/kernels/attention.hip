@@ -28,87 +28,18 @@
 #include <cstdint>
 
 #include "cinn_hip_runtime.h"
-#include "kernels/flex_tile.h"
+#include "kernels/attention_tile.h"
 #include "runtime/hip_check.h"
 
 namespace {
 
-using cinn_hip_kernels::flex::bf16x8;
-using cinn_hip_kernels::flex::f16x8;
-using cinn_hip_kernels::flex::f32x16;
-using cinn_hip_kernels::flex::f32x4;
-using cinn_hip_kernels::flex::LoadAny;
-using cinn_hip_kernels::flex::s16x4;
-using cinn_hip_kernels::flex::u32x4;
-
-// [b][h][t][d] in any order of the first three: d is contiguous
-struct Rows {
-  const void* base;
-  int64_t batch, head, row;  // strides in elements
-};
+using namespace cinn_hip_kernels::attention;
 
 struct AttentionParams {
   Rows q, k[2], v[2], o;
   int heads, bh, tq, t1, t2, d;
   int q_tiles;
   float scale;
-};
-
-template <typename T>
-__device__ __forceinline__ const char* HeadOf(const Rows& r, int b, int h) {
-  return static_cast<const char*>(r.base) + (b * r.batch + h * r.head) * (int64_t)sizeof(T);
-}
-
-// exp(|scale| (s - m)); the scale's sign has gone into the query (a scale of 0 too: there the query is zero and the
-// factor 1, since 0 * -inf of a maximum not yet found or of a masked key is no number).  Full accuracy for fp32; v_exp_f32 (2^-22 or so) of one
-// fused multiply-add where the result is rounded to 16 bits anyway.  -inf for m (no finite score so far) must not make
-// -inf - -inf of scores.
-template <typename T>
-struct Exp {
-  float c;
-  __device__ __forceinline__ explicit Exp(float scale) : c(scale == 0.0f ? 1.0f : fabsf(scale) * 1.4426950408889634f) {}
-  __device__ __forceinline__ float Base(float m) const { return m == -__builtin_inff() ? 0.0f : m * c; }
-  __device__ __forceinline__ float operator()(float s, float base) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -base)); }
-};
-template <>
-struct Exp<float> {
-  float c;
-  __device__ __forceinline__ explicit Exp(float scale) : c(scale == 0.0f ? 1.0f : fabsf(scale)) {}
-  __device__ __forceinline__ float Base(float m) const { return m == -__builtin_inff() ? 0.0f : m; }
-  __device__ __forceinline__ float operator()(float s, float base) const { return expf((s - base) * c); }
-};
-
-// a chunk of the query, negated where the scale is negative, zero where it is zero
-template <typename T>
-__device__ __forceinline__ u32x4 Signed(u32x4 v, float scale) {
-  if (scale == 0.0f) return u32x4{0, 0, 0, 0};
-  return scale < 0.0f ? v ^ (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : v;
-}
-
-template <typename T>
-struct Mma;
-template <>
-struct Mma<_Float16> {
-  typedef f16x8 vec8;
-  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
-  }
-};
-template <>
-struct Mma<__bf16> {
-  typedef bf16x8 vec8;
-  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
-  }
-};
-template <>
-struct Mma<float> {  // four MFMAs of two k each: element e of the lane's chunk is k = e of its half of the wavefront
-  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
-    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], c, 0, 0, 0);
-    return c;
-  }
 };
 
 // One tile of keys or values on its way to LDS: [KT][PITCH bytes], rows beyond the keys and chunks beyond d are zero.

@@ -1,0 +1,302 @@
+// Device code shared by the attention kernels (attention.hip, packed_attention.hip, cached_attention.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "kernels/flex_tile.h"
+
+namespace cinn_hip_kernels {
+namespace attention {
+
+using flex::bf16x8;
+using flex::f16x8;
+using flex::f32x16;
+using flex::f32x4;
+using flex::LoadAny;
+using flex::s16x4;
+using flex::u32x4;
+
+// [b][h][t][d] in any order of the first three: d is contiguous
+struct Rows {
+  const void* base;
+  int64_t batch, head, row;  // strides in elements
+};
+
+template <typename T>
+__device__ __forceinline__ const char* HeadOf(const Rows& r, int b, int h) {
+  return static_cast<const char*>(r.base) + (b * r.batch + h * r.head) * (int64_t)sizeof(T);
+}
+
+// exp(|scale| (s - m)); the scale's sign has gone into the query (a scale of 0 too: there the query is zero and the
+// factor 1, since 0 * -inf of a maximum not yet found or of a masked key is no number).  Full accuracy for fp32; v_exp_f32 (2^-22 or so) of one
+// fused multiply-add where the result is rounded to 16 bits anyway.  -inf for m (no finite score so far) must not make
+// -inf - -inf of scores.
+template <typename T>
+struct Exp {
+  float c;
+  __device__ __forceinline__ explicit Exp(float scale) : c(scale == 0.0f ? 1.0f : fabsf(scale) * 1.4426950408889634f) {}
+  __device__ __forceinline__ float Base(float m) const { return m == -__builtin_inff() ? 0.0f : m * c; }
+  __device__ __forceinline__ float operator()(float s, float base) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -base)); }
+};
+template <>
+struct Exp<float> {
+  float c;
+  __device__ __forceinline__ explicit Exp(float scale) : c(scale == 0.0f ? 1.0f : fabsf(scale)) {}
+  __device__ __forceinline__ float Base(float m) const { return m == -__builtin_inff() ? 0.0f : m; }
+  __device__ __forceinline__ float operator()(float s, float base) const { return expf((s - base) * c); }
+};
+
+// a chunk of the query, negated where the scale is negative, zero where it is zero
+template <typename T>
+__device__ __forceinline__ u32x4 Signed(u32x4 v, float scale) {
+  if (scale == 0.0f) return u32x4{0, 0, 0, 0};
+  return scale < 0.0f ? v ^ (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : v;
+}
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<_Float16> {
+  typedef f16x8 vec8;
+  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<__bf16> {
+  typedef bf16x8 vec8;
+  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<float> {  // four MFMAs of two k each: element e of the lane's chunk is k = e of its half of the wavefront
+  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// How [keys][d] tiles lie in LDS.  K rows are read 16 bytes per lane, rows over lanes: an odd number of 16-byte chunks.  V
+// rows: the four rows of a transposing read, 64 bytes each, fall into different quarters of the banks; single floats: rows
+// four apart do.
+template <typename T, int D>
+struct Layout {
+  static constexpr bool F32    = sizeof(T) == 4;
+  static constexpr int NC      = D * (int)sizeof(T) / 16;  // 16-byte chunks per row
+  static constexpr int DT      = (D + 31) / 32;            // 32-row results of O^T
+  static constexpr int K_PITCH = NC * 16 + 16;
+  static constexpr int V_PITCH = F32 ? DT * 128 + 32 : (DT * 64) % 128 == 64 ? DT * 64 : DT * 64 + 64;
+};
+
+// the bits of a word of 32 keys below `count`
+__device__ __forceinline__ unsigned Below(int count) { return count >= 32 ? ~0u : count <= 0 ? 0u : (1u << count) - 1; }
+
+// 32 queries of a wavefront, a lane of either half holding one: S^T = K Q^T leaves the lane 16 scores of its query, register
+// r of key 8 (r / 4) + 4 half + r % 4, and O^T = V^T P^T sixteen sums of each 32 elements of d in the same order.
+template <typename T, int D>
+struct Queries {
+  typedef Layout<T, D> L;
+  u32x4 q[L::NC / 2];  // chunks 2 i + half of the query's row
+  float m, l;          // l: of this lane's keys only
+  f32x16 o[L::DT];
+
+  __device__ __forceinline__ void Start(const char* row, int chunks, int half, float scale) {
+#pragma unroll
+    for (int i = 0; i < L::NC / 2; ++i) {
+      q[i] = u32x4{0, 0, 0, 0};
+      if (2 * i + half < chunks) q[i] = Signed<T>(LoadAny<T>(row + (2 * i + half) * 16), scale);
+    }
+    m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+    for (int t = 0; t < L::DT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[t][r] = 0.0f;
+  }
+
+  // scores of 32 keys whose rows lie at `tile`
+  __device__ __forceinline__ f32x16 Scores(const char* tile, int lane) const {
+    f32x16 s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+    const char* row = tile + (lane & 31) * L::K_PITCH + (lane >> 5) * 16;
+#pragma unroll
+    for (int i = 0; i < L::NC / 2; ++i) s = Mma<T>::mma(*reinterpret_cast<const u32x4*>(row + i * 32), q[i], s);
+    return s;
+  }
+
+  // scores of keys that the lane's query does not attend to count nothing
+  static __device__ __forceinline__ void Mask(f32x16& s, unsigned word, int lane) {
+    word >>= 4 * (lane >> 5);
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (!((word >> (8 * (r >> 2) + (r & 3))) & 1)) s[r] = -__builtin_inff();
+  }
+
+  // scores -> probabilities against the running maximum; what has been summed is rescaled only when a maximum has grown by
+  // more than a factor of 2^8 (fp32, whose exponent is natural: e^8): probabilities up to 256 (2981) lose nothing in either
+  // type, and after the first tiles few maxima grow that much
+  __device__ __forceinline__ void Soften(f32x16& s, const Exp<T>& ex) {
+    float top = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+    top = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+    if (__ballot((top - m) * ex.c > 8.0f)) {
+      const float keep = ex(m, ex.Base(top));
+      l *= keep;
+#pragma unroll
+      for (int t = 0; t < L::DT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[t][r] *= keep;
+      m = top;
+    }
+    const float base = ex.Base(m);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] = ex(s[r], base);
+      l += s[r];
+    }
+  }
+
+  // sums of 32 keys' values; 16-bit probabilities are rounded on their way into the matrix cores: half a step of the type,
+  // which the result's own rounding has too, at twice (fp16, bf16) the rate that fp32 operands split in two would have
+  __device__ __forceinline__ void Add(const f32x16& s, const char* tile, int lane) {
+    const int half = lane >> 5;
+    if constexpr (L::F32) {
+#pragma unroll
+      for (int t = 0; t < L::DT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = 8 * (r >> 2) + 4 * half + (r & 3);
+          const float v = *reinterpret_cast<const float*>(tile + key * L::V_PITCH + (t * 32 + (lane & 31)) * 4);
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[r], o[t], 0, 0, 0);
+        }
+    } else {
+      typedef T vec8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        vec8 pr;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pr[e] = (T)s[8 * g + e];
+#pragma unroll
+        for (int t = 0; t < L::DT; ++t) {
+          // four keys x sixteen d per group of 16 lanes, transposed on the way
+          s16x4 part[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const char* at = tile + (16 * g + 8 * u + 4 * half + ((lane & 15) >> 2)) * L::V_PITCH +
+                             (32 * t + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+            part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)at);
+          }
+          o[t] = Mma<T>::mma(__builtin_bit_cast(u32x4, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7)),
+                             __builtin_bit_cast(u32x4, pr), o[t]);
+        }
+      }
+    }
+  }
+
+  // whether one of the 32 keys' values is infinite or no number
+  static __device__ __forceinline__ bool Unbounded(const char* tile, int chunks, int lane) {
+    constexpr unsigned kExponent = L::F32 ? 0x7f800000u : sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
+    bool found = false;
+    for (int at = lane; at < 32 * chunks; at += 64) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(tile + at / chunks * L::V_PITCH + at % chunks * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        found |= (v[e] & kExponent) == kExponent;
+        if (!L::F32) found |= (v[e] >> 16 & kExponent) == kExponent;
+      }
+    }
+    return __ballot(found) != 0;
+  }
+
+  // Add for values among which are infinities or NaN, where a probability of zero by the mask must not make 0 * inf: key
+  // by key, only where the query attends to it
+  __device__ __forceinline__ void AddChosen(const f32x16& s, unsigned word, const char* tile, int lane) {
+    const int half = lane >> 5;
+#pragma unroll 1
+    for (int at = 0; at < 32; ++at) {
+      const int owner = at >> 4, reg = at & 15, key = 8 * (reg >> 2) + 4 * owner + (reg & 3);
+      float mine = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mine = reg == r ? s[r] : mine;
+      mine = (float)(T)mine;
+      const float other = __shfl_xor(mine, 32), prob = half == owner ? mine : other;
+      const bool chosen = (word >> key) & 1;
+      const T* row      = reinterpret_cast<const T*>(tile + key * L::V_PITCH) + 4 * half;
+#pragma unroll
+      for (int t = 0; t < L::DT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float v = (float)row[32 * t + 8 * (r >> 2) + (r & 3)];
+          o[t][r]       = chosen ? __builtin_fmaf(prob, v, o[t][r]) : o[t][r];
+        }
+    }
+  }
+
+  // one step: 32 keys of which the lane's query attends to those in `word`
+  __device__ __forceinline__ void Step(const char* k_tile, const char* v_tile, unsigned word, int chunks, const Exp<T>& ex, int lane) {
+    f32x16 s = Scores(k_tile, lane);
+    const bool masked = __ballot(word != ~0u) != 0;
+    if (masked) Mask(s, word, lane);
+    Soften(s, ex);
+    if (masked && Unbounded(v_tile, chunks, lane)) {
+      AddChosen(s, word, v_tile, lane);
+    } else {
+      Add(s, v_tile, lane);
+    }
+  }
+
+  // what another wavefront has of the same queries, [register][lane]
+  static constexpr int kRegisters = L::DT * 16 + 2;
+  __device__ __forceinline__ void Hand(float* to, int lane) const {
+#pragma unroll
+    for (int t = 0; t < L::DT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) to[(t * 16 + r) * 64 + lane] = o[t][r];
+    to[(kRegisters - 2) * 64 + lane] = m;
+    to[(kRegisters - 1) * 64 + lane] = l;
+  }
+  __device__ __forceinline__ void Join(const float* from, const Exp<T>& ex, int lane) {
+    const float m2 = from[(kRegisters - 2) * 64 + lane], top = fmaxf(m, m2), base = ex.Base(top);
+    const float keep = ex(m, base), add = ex(m2, base);
+    l = l * keep + from[(kRegisters - 1) * 64 + lane] * add;
+#pragma unroll
+    for (int t = 0; t < L::DT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[t][r] = o[t][r] * keep + from[(t * 16 + r) * 64 + lane] * add;
+    m = top;
+  }
+
+  // o times `factor` to the query's row of the result
+  __device__ __forceinline__ void Store(char* row, int d, float factor, int half) const {
+#pragma unroll
+    for (int t = 0; t < L::DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = t * 32 + 8 * i + 4 * half;
+        T four[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) four[e] = (T)(o[t][4 * i + e] * factor);
+        if (at < d) __builtin_memcpy(row + at * sizeof(T), four, sizeof(four));
+      }
+  }
+};
+
+// v / d for 0 <= v < 2^31 and 1 <= d < 2^31, by a product: m = ceil(2^(31 + s) / d) with 2^s >= d is below 2^32 and off by less
+// than d / 2^(31 + s), so v m / 2^(31 + s) is off by less than 1 / d
+struct Divisor {
+  unsigned multiplier;
+  int shift, value;
+  __host__ explicit Divisor(int d = 1) : shift(0), value(d) {
+    while ((int64_t{1} << shift) < d) ++shift;
+    multiplier = (unsigned)(((uint64_t{1} << (31 + shift)) + d - 1) / d);
+  }
+  __device__ __forceinline__ int operator()(int v) const { return (int)((uint64_t)(unsigned)v * multiplier >> (31 + shift)); }
+};
+
+}  // namespace attention
+}  // namespace cinn_hip_kernels

@@ -252,6 +252,22 @@ class NetBuilder(object):
                            global_pooling=global_pooling, data_format=data_format, adaptive=adaptive,
                            padding_algorithm=padding_algorithm)
 
+    @staticmethod
+    def _attention_options(q, scale, heads, kv_heads, q_head, k_head, v_head):
+        return dict(scale=float(q.shape()[-1] ** -0.5 if scale is None else scale), heads=int(heads), kv_heads=int(kv_heads),
+                    q_head=int(q_head), k_head=int(k_head), v_head=int(v_head))
+
+    def packed_attention(self, q, k, v, offsets, scale=None, heads=0, kv_heads=0, q_head=0, k_head=0, v_head=0):
+        """Causal attention of whole prompts of different lengths, packed behind one another: sequence s is the rows
+        offsets[s] .. offsets[s + 1] - 1 (int32, data of the program) of q, k and v [tokens, their heads, d], and each of its
+        rows attends to the rows of its sequence up to itself.  Returns [tokens, heads, d], zero in rows of no sequence.
+
+        `heads` query heads from `q_head` on share `kv_heads` key and value heads from `k_head` and `v_head` on, heads /
+        kv_heads neighbours each (0: all heads from there on); packed projections are passed as q, k and v alike.  `scale`
+        defaults to d ** -0.5.  fp16, bf16 or fp32, d at most 128 and a multiple of 16 bytes."""
+        return self._call1("PackedAttention", [q, k, v, offsets],
+                           **self._attention_options(q, scale, heads, kv_heads, q_head, k_head, v_head))
+
     def _rotary(self, method, x, positions, heads, rotary_dim, interleaved, theta, factor, original_length, low, high, magnitude):
         wide = dict(theta=theta, factor=factor, low=low, high=high, magnitude=magnitude)
         return self._call1(method, [x, positions], heads=int(heads), rotary_dim=int(rotary_dim), interleaved=bool(interleaved),

@@ -281,6 +281,19 @@ void cinn_call_hip_top_k(void* v_args, int num_args, int outer, int size, int in
 void cinn_call_hip_attention(void* v_args, int num_args, float scale, int batch, int heads, int queries, int keys,
                              int appended, int d, int operands, int layouts, int parts, void* stream);
 
+/* Causal attention over packed sequences: sequence s of `sequences` holds the rows offsets[s] .. offsets[s + 1] - 1 of q, k, v
+ * and out; row t of it attends to its rows up to t, out = softmax(scale q k^T) v with the conventions of
+ * cinn_call_hip_attention, and query head h reads key and value head h / (heads / kv_heads).  q, k and v are
+ * [tokens][their heads][d], of which `heads` from q_head and `kv_heads` from k_head and v_head on are meant; out is
+ * [tokens][heads][d].  Rows before offsets[0] and from offsets[sequences] on belong to no sequence: out is zero there.
+ * Keys and values that a row does not attend to, infinities and NaN among them, do not count.  offsets: int32
+ * [sequences + 1], in order, read on the GPU; with offsets out of order or range results are unspecified, accesses in
+ * bounds.  fp16 / bf16 / fp32; d at most 128, a multiple of 16 bytes.  operands: four bits for each of the slots q, k, v,
+ * offsets, which input it is; v_args = {inputs..., out}.  No counterpart in the reference. */
+void cinn_call_hip_packed_attention(void* v_args, int num_args, float scale, int tokens, int sequences, int heads, int kv_heads,
+                                    int d, int operands, int q_heads, int q_head, int k_heads, int k_head, int v_heads, int v_head,
+                                    void* stream);
+
 /* Rotary positions: y [tokens][heads][d] from the first `heads` heads of x [tokens][total_heads][d]; fp16 / bf16 / fp32, positions
  * [tokens] int32 or int64.  Pair i < rotary_dim / 2 of a head, its elements 2 i and 2 i + 1 (interleaved) or i and
  * i + rotary_dim / 2, is turned by position * f_i and multiplied by magnitude, f_i = theta^(-2 i / rotary_dim) scaled:
