@@ -202,6 +202,11 @@ const std::map<std::string, Method>& Methods() {
     m["PackedAttention"] = [=](NetBuilder& b, const std::vector<Variable>& in, const AttributeMap& a) {
       return std::vector<Variable>{b.PackedAttention(in.at(0), in.at(1), in.at(2), in.at(3), attention_options(a))};
     };
+    m["CachedAttention"] = [=](NetBuilder& b, const std::vector<Variable>& in, const AttributeMap& a) {
+      return std::vector<Variable>{b.CachedAttention(in.at(0), in.at(1), in.at(2), in.at(3), in.at(4), in.at(5), in.at(6),
+                                                     in.size() > 7 ? in[7] : Variable(), GetAttr<std::string>(a, "page_layout", "row_head"),
+                                                     attention_options(a))};
+    };
     auto rotary_options = [](const AttributeMap& a) {
       NetBuilder::RotaryOptions o;
       o.rotary_dim      = GetAttr<int>(a, "rotary_dim", o.rotary_dim);

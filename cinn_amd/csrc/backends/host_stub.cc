@@ -91,6 +91,10 @@ void InvokePackedAttention(const std::vector<BakedArg>& a, void* args, int32_t n
   cinn_call_hip_packed_attention(args, n, F(a[2]), I(a[3]), I(a[4]), I(a[5]), I(a[6]), I(a[7]), I(a[8]), I(a[9]), I(a[10]), I(a[11]),
                                  I(a[12]), I(a[13]), I(a[14]), stream);
 }
+void InvokeCachedAttention(const std::vector<BakedArg>& a, void* args, int32_t n, void* stream) {
+  cinn_call_hip_cached_attention(args, n, F(a[2]), I(a[3]), I(a[4]), I(a[5]), I(a[6]), I(a[7]), I(a[8]), I(a[9]), I(a[10]), I(a[11]),
+                                 I(a[12]), I(a[13]), I(a[14]), I(a[15]), I(a[16]), I(a[17]), I(a[18]), stream);
+}
 void InvokeRotaryEmbedding(const std::vector<BakedArg>& a, void* args, int32_t n, void* stream) {
   cinn_call_hip_rotary_embedding(args, n, I(a[2]), I(a[3]), I(a[4]), I(a[5]), I(a[6]), I(a[7]), I(a[8]), D(a[9]), D(a[10]), I(a[11]),
                                  D(a[12]), D(a[13]), D(a[14]), stream);
@@ -147,6 +151,9 @@ ExternApiRegistry::ExternApiRegistry() {
   // (kernel_args, kernel_args_num, scale, tokens, sequences, heads, kv_heads, d, operands, heads of q and the first in use, of
   // k, of v, kernel_stream)
   Register("cinn_call_hip_packed_attention", InvokePackedAttention, 16);
+  // (kernel_args, kernel_args_num, scale, batch, tokens, heads, kv_heads, d, pages, page_rows, page_layout, columns, operands,
+  // heads of q and the first in use, of k, of v, kernel_stream)
+  Register("cinn_call_hip_cached_attention", InvokeCachedAttention, 20);
   // (kernel_args, kernel_args_num, tokens, heads, total_heads, d, rotary_dim, interleaved, transposed, theta, factor,
   // original_length, low, high, magnitude, kernel_stream)
   Register("cinn_call_hip_rotary_embedding", InvokeRotaryEmbedding, 16);

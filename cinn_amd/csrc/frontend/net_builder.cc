@@ -327,6 +327,15 @@ Variable NetBuilder::PackedAttention(const Variable& q, const Variable& k, const
                                      const AttentionOptions& options) {
   return CustomInstr("packed_attention", {q, k, v, offsets}, AttentionAttrs(options)).front();
 }
+Variable NetBuilder::CachedAttention(const Variable& q, const Variable& k, const Variable& v, const Variable& k_pages,
+                                     const Variable& v_pages, const Variable& table, const Variable& lengths, const Variable& parents,
+                                     const std::string& page_layout, const AttentionOptions& options) {
+  auto attrs           = AttentionAttrs(options);
+  attrs["page_layout"] = page_layout;
+  std::vector<Variable> inputs{q, k, v, k_pages, v_pages, table, lengths};
+  if (parents.defined()) inputs.push_back(parents);
+  return CustomInstr("cached_attention", inputs, attrs).front();
+}
 
 namespace {
 utils::AttributeMap RotaryAttrs(int heads, const NetBuilder::RotaryOptions& o, bool transposed) {

@@ -123,6 +123,11 @@ class NetBuilder {
   };
   // causal, over sequences packed behind one another in [tokens, heads, d] (cinn_call_hip_packed_attention)
   Variable PackedAttention(const Variable& q, const Variable& k, const Variable& v, const Variable& offsets, const AttentionOptions& options);
+  // new tokens [batch, tokens, heads, d] over a paged cache and each other (cinn_call_hip_cached_attention); parents may be an
+  // undefined Variable; page_layout "row_head" or "head_row"
+  Variable CachedAttention(const Variable& q, const Variable& k, const Variable& v, const Variable& k_pages, const Variable& v_pages,
+                           const Variable& table, const Variable& lengths, const Variable& parents, const std::string& page_layout,
+                           const AttentionOptions& options);
   // Rotary positions of the first `heads` heads (0: all) of x [..., heads, d] at positions [...], rotary_dim elements of each
   // (0: all), and x's gradient from dy of y's shape; theta, scaling and the order of pairs as in
   // cinn_call_hip_rotary_embedding.  No counterpart in the reference.

@@ -1651,6 +1651,17 @@ ir::LoweredFuncRef OpLowerer::LowerLibraryCall(const Group& group) const {
     args.push_back(Expr(GetAttr<float>(n->attrs, "scale", 1.0f)));
     push_ints({q[0], n->inputs[3]->shape[0] - 1, all, AttentionKvHeads(n->inputs[1]->shape[1], n->attrs), q[2], operand_slots()});
     push_attention_heads();
+  } else if (op == "cached_attention") {
+    api               = "cinn_call_hip_cached_attention";
+    const auto& q     = n->inputs[0]->shape;
+    const auto& pages = n->inputs[3]->shape;
+    const bool by_row = GetAttr<std::string>(n->attrs, "page_layout", "row_head") == "row_head";
+    check_rows();
+    args.push_back(Expr(GetAttr<float>(n->attrs, "scale", 1.0f)));
+    push_ints({q[0], q[1], n->outputs[0]->shape[2], AttentionKvHeads(n->inputs[1]->shape[2], n->attrs), q[3]});
+    push_ints({pages[0], by_row ? pages[1] : pages[2], by_row ? 0 : 1, n->inputs[5]->shape[1]});
+    push_ints({operand_slots() | (n->inputs.size() == 7 ? static_cast<int>(15u << 28) : 0)});
+    push_attention_heads();
   } else if (op == "rotary_embedding") {
     api           = "cinn_call_hip_rotary_embedding";
     const auto& x = n->inputs[0]->shape;

@@ -840,6 +840,31 @@ OpRegistry::OpRegistry() {
     op.infer_dtype = [](const std::vector<Type>& in, const AttributeMap&) { return std::vector<Type>{AttentionType("packed_attention", in, 3)}; };
   }
   {
+    // q, k, v [batch, tokens, heads, d] of new tokens, the pages of a cache of keys and of values, which pages a sequence has and
+    // how many rows in them, and the new tokens' parents or not
+    auto& op       = r->Register("cached_attention");
+    op.pattern     = OpPatternKind::kNonFusible;
+    op.num_inputs  = -1;
+    op.infer_shape = [](const std::vector<ShapeType>& in, const AttributeMap& a) {
+      CINN_CHECK(in.size() == 7 || in.size() == 8) << "cached_attention: q, k, v, the pages of both, table, lengths and parents or not are expected";
+      const ShapeType out = AttentionShape("cached_attention", in, a, 4);
+      CINN_CHECK_LE(out[1], 64) << "cached_attention: at most 64 new tokens of a sequence";
+      const std::string layout = GetAttr<std::string>(a, "page_layout", "row_head");
+      CINN_CHECK(layout == "row_head" || layout == "head_row") << "cached_attention: page_layout " << layout << " is neither row_head nor head_row";
+      CINN_CHECK(in[3] == in[4] && in[3].size() == 4) << "cached_attention: k_pages and v_pages are of one shape of rank 4";
+      const int kv_heads = AttentionKvHeads(in[1][2], a);
+      CINN_CHECK(in[3][layout == "row_head" ? 2 : 1] == kv_heads && in[3][3] == out[3])
+          << "cached_attention: pages of " << kv_heads << " heads of " << out[3] << " elements are expected";
+      CINN_CHECK(in[5].size() == 2 && in[5][0] == out[0]) << "cached_attention: a row of table for every sequence is expected";
+      const int64_t capacity = static_cast<int64_t>(in[5][1]) * in[3][layout == "row_head" ? 1 : 2];
+      CINN_CHECK(capacity < (int64_t{1} << 30)) << "cached_attention: " << capacity << " rows per sequence are too many";
+      CINN_CHECK(in[6] == ShapeType{out[0]}) << "cached_attention: a length for every sequence is expected";
+      if (in.size() == 8) CINN_CHECK(in[7] == (ShapeType{out[0], out[1]})) << "cached_attention: a parent for every token is expected";
+      return std::vector<ShapeType>{out};
+    };
+    op.infer_dtype = [](const std::vector<Type>& in, const AttributeMap&) { return std::vector<Type>{AttentionType("cached_attention", in, 5)}; };
+  }
+  {
     // x [..., total heads, d], positions [...] -> the first `heads` heads (0: all), turned by their positions; transposed: the
     // gradient
     auto& op       = r->Register("rotary_embedding");

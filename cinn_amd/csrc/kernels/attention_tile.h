@@ -291,7 +291,7 @@ struct Queries {
 struct Divisor {
   unsigned multiplier;
   int shift, value;
-  __host__ explicit Divisor(int d = 1) : shift(0), value(d) {
+  __host__ Divisor(int d = 1) : shift(0), value(d) {
     while ((int64_t{1} << shift) < d) ++shift;
     multiplier = (unsigned)(((uint64_t{1} << (31 + shift)) + d - 1) / d);
   }

@@ -268,6 +268,22 @@ class NetBuilder(object):
         return self._call1("PackedAttention", [q, k, v, offsets],
                            **self._attention_options(q, scale, heads, kv_heads, q_head, k_head, v_head))
 
+    def cached_attention(self, q, k, v, k_pages, v_pages, table, lengths, parents=None, scale=None, heads=0, kv_heads=0,
+                         q_head=0, k_head=0, v_head=0, page_layout="row_head"):
+        """Attention of new tokens, q, k and v [batch, tokens, their heads, d] with at most 64 tokens a sequence, over a paged
+        cache and each other; returns [batch, tokens, heads, d].  The cache is read, not written.
+
+        Every token attends to the cached rows 0 .. lengths[b] - 1 of its sequence, to itself and to its ancestors among the
+        new tokens: without `parents` to all before it, with parents [batch, tokens] to a tree of drafted tokens, parents[b][i]
+        < i being the token that i follows, -1 none; a token with another parent is padding, its result zero, and nothing
+        attends to it.  Row r of sequence b is row r % page of page table[b][r // page]; k_pages and v_pages are [pages, page,
+        kv_heads, d] ("row_head") or [pages, kv_heads, page, d] ("head_row").  table, lengths and parents are int32 and data of
+        the program, which serves caches of every length; a length is taken between 0 and what the table can hold, and a page
+        number that is none holds no rows.  Heads, scale and types as in packed_attention."""
+        inputs = [q, k, v, k_pages, v_pages, table, lengths] + ([] if parents is None else [parents])
+        return self._call1("CachedAttention", inputs, page_layout=str(page_layout),
+                           **self._attention_options(q, scale, heads, kv_heads, q_head, k_head, v_head))
+
     def _rotary(self, method, x, positions, heads, rotary_dim, interleaved, theta, factor, original_length, low, high, magnitude):
         wide = dict(theta=theta, factor=factor, low=low, high=high, magnitude=magnitude)
         return self._call1(method, [x, positions], heads=int(heads), rotary_dim=int(rotary_dim), interleaved=bool(interleaved),

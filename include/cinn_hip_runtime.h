@@ -294,6 +294,21 @@ void cinn_call_hip_packed_attention(void* v_args, int num_args, float scale, int
                                     int d, int operands, int q_heads, int q_head, int k_heads, int k_head, int v_heads, int v_head,
                                     void* stream);
 
+/* Attention of `tokens` new tokens of each of `batch` sequences (at most 64) over a paged cache and each other: token i of
+ * sequence b attends to the cached rows 0 .. lengths[b] - 1, to itself and to its ancestors among the new tokens, parents[b][i]
+ * < i being the one before it, -1 none.  A token with any other parent is no token: its out is zero and nothing attends to it.
+ * Without parents (slot 15) every token follows the one before.  q, k, v [batch][tokens][their heads][d] and out [batch]
+ * [tokens][heads][d], heads and scale as in cinn_call_hip_packed_attention.  The cache: k and v pages, [pages][page_rows]
+ * [kv_heads][d] (page_layout 0) or [pages][kv_heads][page_rows][d] (1); row r of sequence b lies in page table[b][r /
+ * page_rows] of table [batch][columns].  lengths are taken between 0 and columns * page_rows; a page number out of range
+ * holds no rows.  table, lengths and parents are int32, read on the GPU.  fp16 / bf16 / fp32; d at most 128, a multiple of 16
+ * bytes.  operands: four bits for each of the slots q, k, v, k pages, v pages, table, lengths, parents, which input it is;
+ * v_args = {inputs..., out}.  Long caches are divided over blocks by way of the stream's split-K scratch
+ * (cinn_hip_scratch_reserve); under capture with too little of it, over fewer.  No counterpart in the reference. */
+void cinn_call_hip_cached_attention(void* v_args, int num_args, float scale, int batch, int tokens, int heads, int kv_heads, int d,
+                                    int pages, int page_rows, int page_layout, int columns, int operands, int q_heads, int q_head,
+                                    int k_heads, int k_head, int v_heads, int v_head, void* stream);
+
 /* Rotary positions: y [tokens][heads][d] from the first `heads` heads of x [tokens][total_heads][d]; fp16 / bf16 / fp32, positions
  * [tokens] int32 or int64.  Pair i < rotary_dim / 2 of a head, its elements 2 i and 2 i + 1 (interleaved) or i and
  * i + rotary_dim / 2, is turned by position * f_i and multiplied by magnitude, f_i = theta^(-2 i / rotary_dim) scaled:

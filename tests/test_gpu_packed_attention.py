@@ -1,13 +1,6 @@
 """packed_attention (packed_attention.hip) against float64 at the edges of its tiles - 32 pairs of query and head per
 wavefront, 32 to 256 per block, 32 keys per step - with empty sequences and single rows among the others, heads that share
-keys, operands out of packed projections, rows of no sequence, infinities and NaN where nothing attends to them.
-
-Bounds: a score is an fp32 sum of d products (2^-24 sqrt(d) + 2^-22 of the products' magnitudes); the relative error of a
-probability is twice that and what exp adds (its argument's rounding, 2^-24 of up to 32, and its own 2^-21), together
-under 2^-18.  16-bit operands of the second product are rounded probabilities (half a step, subnormal ones 2^-25), as are
-their sums' (another half); the result rounds once."""
-import math
-
+keys, operands out of packed projections, rows of no sequence, infinities and NaN where nothing attends to them."""
 import numpy as np
 import pytest
 
@@ -16,29 +9,9 @@ from cinn_amd.common import DefaultAMDGPUTarget, Int
 from cinn_amd.frontend import Computation, NetBuilder
 
 from helpers import run
-from typed_inputs import TYPES, ULP, as_float64, assert_within, dtype, normal, rounded
+from typed_inputs import TYPES, as_float64, assert_within, attend, dtype, normal, rounded
 
 pytestmark = pytest.mark.gpu
-
-
-def attend(q, k, v, allowed, scale, kind):
-    """one head: float64 result and the bound on its error; what is not allowed is left out"""
-    out, bound = np.zeros(q.shape), np.zeros(q.shape)
-    u = ULP[kind]
-    for i in range(q.shape[0]):
-        kk, vv = k[allowed[i]], v[allowed[i]]
-        if not len(kk):
-            continue
-        with np.errstate(invalid="ignore", over="ignore"):
-            s = scale * (kk @ q[i])
-            p = np.exp(s - s.max())
-            p /= p.sum()
-            out[i] = p @ vv
-            score = (2.0 ** -24 * math.sqrt(q.shape[1]) + 2.0 ** -22) * abs(scale) * (np.abs(kk) @ np.abs(q[i])).max()
-            bound[i] = (2 * score + 2.0 ** -18 + 2 * u) * (p @ np.abs(vv)) + u * np.abs(out[i])
-            if kind == "float16":
-                bound[i] += len(kk) * 2.0 ** -25 * np.abs(vv).max() + 2.0 ** -24
-    return out, bound
 
 
 def causal(q, k, v, offsets, scale, kind):

@@ -1,4 +1,6 @@
-"""Inputs in a floating type and their values in float64 (not collected)."""
+"""Inputs in a floating type, their values in float64, and attention of one head in float64 (not collected)."""
+import math
+
 import numpy as np
 
 from cinn_amd.common import BFloat16, Float, bfloat16_bits_to_float32, float32_to_bfloat16_bits
@@ -37,3 +39,27 @@ def assert_within(got, want, bound, kind):
     assert got.shape == want.shape and over.max() <= 0, "%d of %d out of bounds, the worst by %g at %s: %r, wanted %r +- %r" % (
         (over > 0).sum(), over.size, over.max(), np.unravel_index(over.argmax(), over.shape),
         as_float64(got, kind).flat[over.argmax()], want.flat[over.argmax()], np.broadcast_to(bound, want.shape).flat[over.argmax()])
+
+
+def attend(q, k, v, allowed, scale, kind):
+    """float64 result and the bound on its error; what is not allowed is left out.  A score is an fp32 sum of d products (2^-24
+    sqrt(d) + 2^-22 of the products' magnitudes); the relative error of a probability is twice that and what exp adds (its
+    argument's rounding, 2^-24 of up to 32, and its own 2^-21), together under 2^-18.  16-bit operands of the second product
+    are rounded probabilities (half a step, subnormal ones 2^-25), as are their sums' (another half); the result rounds
+    once."""
+    out, bound = np.zeros(q.shape), np.zeros(q.shape)
+    u = ULP[kind]
+    for i in range(q.shape[0]):
+        kk, vv = k[allowed[i]], v[allowed[i]]
+        if not len(kk):
+            continue
+        with np.errstate(invalid="ignore", over="ignore"):
+            s = scale * (kk @ q[i])
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            out[i] = p @ vv
+            score = (2.0 ** -24 * math.sqrt(q.shape[1]) + 2.0 ** -22) * abs(scale) * (np.abs(kk) @ np.abs(q[i])).max()
+            bound[i] = (2 * score + 2.0 ** -18 + 2 * u) * (p @ np.abs(vv)) + u * np.abs(out[i])
+            if kind == "float16":
+                bound[i] += len(kk) * 2.0 ** -25 * np.abs(vv).max() + 2.0 ** -24
+    return out, bound
