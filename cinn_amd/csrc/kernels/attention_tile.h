@@ -80,16 +80,40 @@ struct Mma<float> {  // four MFMAs of two k each: element e of the lane's chunk 
   }
 };
 
-// How [keys][d] tiles lie in LDS.  K rows are read 16 bytes per lane, rows over lanes: an odd number of 16-byte chunks.  V
-// rows: the four rows of a transposing read, 64 bytes each, fall into different quarters of the banks; single floats: rows
-// four apart do.
+// How [keys][d] tiles lie in LDS: KAt(row, c) is where chunk c of a key's row starts, VAt(row, c) of a value's.
 template <typename T, int D>
-struct Layout {
-  static constexpr bool F32    = sizeof(T) == 4;
-  static constexpr int NC      = D * (int)sizeof(T) / 16;  // 16-byte chunks per row
-  static constexpr int DT      = (D + 31) / 32;            // 32-row results of O^T
+struct Shape {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int NC   = D * (int)sizeof(T) / 16;  // 16-byte chunks per row
+  static constexpr int DT   = (D + 31) / 32;            // 32-row results of O^T
+};
+
+// Rows apart, for tiles that are stored from registers.  K rows are read 16 bytes per lane, rows over lanes: an odd number of
+// 16-byte chunks.  V rows: the four rows of a transposing read, 64 bytes each, fall into different quarters of the banks;
+// single floats: rows four apart do.
+template <typename T, int D>
+struct Padded : Shape<T, D> {
+  using Shape<T, D>::NC, Shape<T, D>::DT, Shape<T, D>::F32;
   static constexpr int K_PITCH = NC * 16 + 16;
   static constexpr int V_PITCH = F32 ? DT * 128 + 32 : (DT * 64) % 128 == 64 ? DT * 64 : DT * 64 + 64;
+  static __device__ __forceinline__ int KAt(int row, int c) { return row * K_PITCH + c * 16; }
+  static __device__ __forceinline__ int VAt(int row, int c) { return row * V_PITCH + c * 16; }
+};
+
+// Rows behind one another, for tiles that loads write to LDS directly, 64 chunks in order per instruction; the chunks of a row
+// change places instead.  K: eight rows' neighbouring chunks, which LDS serves together, lie in different sixteenths of the
+// banks' 256 bytes.  V: four rows' 64 bytes in different quarters; single floats: the halves for rows four apart.
+template <typename T, int D>
+struct Dense : Shape<T, D> {
+  using Shape<T, D>::NC, Shape<T, D>::DT, Shape<T, D>::F32;
+  static constexpr int BYTES = 32 * NC * 16;  // a tile of 32 keys or values
+  static constexpr bool POW2 = (NC & (NC - 1)) == 0;
+  static __device__ __forceinline__ int Turn(int c, int by) { return POW2 ? c ^ by : (c + by >= NC ? c + by - NC : c + by); }
+  static __device__ __forceinline__ int Back(int c, int by) { return POW2 ? c ^ by : (c < by ? c - by + NC : c - by); }
+  static __device__ __forceinline__ int RowTurn(int row) {
+    return NC % 16 == 0 ? 2 * (row & 7) : NC % 8 == 0 ? 2 * ((row >> 1) & 3) : 2 * ((row >> 2) & 1);
+  }
+  static __device__ __forceinline__ int At(int row, int c) { return (row * NC + Turn(c, RowTurn(row))) * 16; }
 };
 
 // the bits of a word of 32 keys below `count`
@@ -97,9 +121,9 @@ __device__ __forceinline__ unsigned Below(int count) { return count >= 32 ? ~0u 
 
 // 32 queries of a wavefront, a lane of either half holding one: S^T = K Q^T leaves the lane 16 scores of its query, register
 // r of key 8 (r / 4) + 4 half + r % 4, and O^T = V^T P^T sixteen sums of each 32 elements of d in the same order.
-template <typename T, int D>
+template <typename T, int D, class Layout = Padded<T, D>>
 struct Queries {
-  typedef Layout<T, D> L;
+  typedef Layout L;
   u32x4 q[L::NC / 2];  // chunks 2 i + half of the query's row
   float m, l;          // l: of this lane's keys only
   f32x16 o[L::DT];
@@ -122,9 +146,9 @@ struct Queries {
     f32x16 s;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = 0.0f;
-    const char* row = tile + (lane & 31) * L::K_PITCH + (lane >> 5) * 16;
 #pragma unroll
-    for (int i = 0; i < L::NC / 2; ++i) s = Mma<T>::mma(*reinterpret_cast<const u32x4*>(row + i * 32), q[i], s);
+    for (int i = 0; i < L::NC / 2; ++i)
+      s = Mma<T>::mma(*reinterpret_cast<const u32x4*>(tile + L::KAt(lane & 31, 2 * i + (lane >> 5))), q[i], s);
     return s;
   }
 
@@ -136,15 +160,15 @@ struct Queries {
       if (!((word >> (8 * (r >> 2) + (r & 3))) & 1)) s[r] = -__builtin_inff();
   }
 
-  // scores -> probabilities against the running maximum; what has been summed is rescaled only when a maximum has grown by
-  // more than a factor of 2^8 (fp32, whose exponent is natural: e^8): probabilities up to 256 (2981) lose nothing in either
-  // type, and after the first tiles few maxima grow that much
+  // scores -> probabilities against the running maximum; what has been summed is rescaled only when a score exceeds it by
+  // more than a factor of 2^8 (fp32, whose exponent is natural: e^8), and only then do the lanes of a query agree on a new
+  // one: probabilities up to 256 (2981) lose nothing in either type, and after the first tiles few maxima grow that much
   __device__ __forceinline__ void Soften(f32x16& s, const Exp<T>& ex) {
     float top = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-    top = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
     if (__ballot((top - m) * ex.c > 8.0f)) {
+      top = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
       const float keep = ex(m, ex.Base(top));
       l *= keep;
 #pragma unroll
@@ -171,7 +195,7 @@ struct Queries {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int key = 8 * (r >> 2) + 4 * half + (r & 3);
-          const float v = *reinterpret_cast<const float*>(tile + key * L::V_PITCH + (t * 32 + (lane & 31)) * 4);
+          const float v = *reinterpret_cast<const float*>(tile + L::VAt(key, t * 8 + (lane & 31) / 4) + (lane & 3) * 4);
           o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[r], o[t], 0, 0, 0);
         }
     } else {
@@ -187,8 +211,8 @@ struct Queries {
           s16x4 part[2];
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const char* at = tile + (16 * g + 8 * u + 4 * half + ((lane & 15) >> 2)) * L::V_PITCH +
-                             (32 * t + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+            const char* at = tile + L::VAt(16 * g + 8 * u + 4 * half + ((lane & 15) >> 2), 4 * t + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) +
+                             (lane & 1) * 8;
             part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)at);
           }
           o[t] = Mma<T>::mma(__builtin_bit_cast(u32x4, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7)),
@@ -203,7 +227,7 @@ struct Queries {
     constexpr unsigned kExponent = L::F32 ? 0x7f800000u : sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
     bool found = false;
     for (int at = lane; at < 32 * chunks; at += 64) {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(tile + at / chunks * L::V_PITCH + at % chunks * 16);
+      const u32x4 v = *reinterpret_cast<const u32x4*>(tile + L::VAt(at / chunks, at % chunks));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         found |= (v[e] & kExponent) == kExponent;
@@ -226,12 +250,13 @@ struct Queries {
       mine = (float)(T)mine;
       const float other = __shfl_xor(mine, 32), prob = half == owner ? mine : other;
       const bool chosen = (word >> key) & 1;
-      const T* row      = reinterpret_cast<const T*>(tile + key * L::V_PITCH) + 4 * half;
 #pragma unroll
       for (int t = 0; t < L::DT; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float v = (float)row[32 * t + 8 * (r >> 2) + (r & 3)];
+          const int byte = (32 * t + 8 * (r >> 2) + 4 * half + (r & 3)) * (int)sizeof(T);
+          if (byte >= L::NC * 16) continue;  // the last 32 elements of a D that is no multiple of 32
+          const float v = (float)*reinterpret_cast<const T*>(tile + L::VAt(key, byte >> 4) + (byte & 15));
           o[t][r]       = chosen ? __builtin_fmaf(prob, v, o[t][r]) : o[t][r];
         }
     }
@@ -297,6 +322,31 @@ struct Divisor {
   }
   __device__ __forceinline__ int operator()(int v) const { return (int)((uint64_t)(unsigned)v * multiplier >> (31 + shift)); }
 };
+
+// Loads from memory straight to LDS: 16 bytes (4 bytes) a lane, written at LDS address `to` + 16 (4) * lane.  Inline assembly,
+// so that the compiler does not track them: tracked, it would wait for all of them before every LDS read.
+__device__ __forceinline__ void CopyToLds16(const void* from, unsigned to) {
+  to = __builtin_amdgcn_readfirstlane(to);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory");
+}
+// from a base that the wavefront shares and a lane's offset
+__device__ __forceinline__ void CopyToLds16(const void* base, unsigned off, unsigned to) {
+  to = __builtin_amdgcn_readfirstlane(to);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void CopyToLds4(const void* from, unsigned to) {
+  to = __builtin_amdgcn_readfirstlane(to);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(from) : "memory");
+}
+__device__ __forceinline__ unsigned LdsAddress(const void* p) {
+  return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+// all but the last N of this wavefront's vector memory instructions have landed
+template <int N>
+__device__ __forceinline__ void WaitForAllBut() {
+  static_assert(N < 64);
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4 << 14));
+}
 
 }  // namespace attention
 }  // namespace cinn_hip_kernels

@@ -87,12 +87,29 @@ __device__ __forceinline__ unsigned long long SeenBy(const CachedParams& p, int 
   return __shfl(word, token);
 }
 
+// What becomes of a run of a unit's tiles: the result where it is all of them, otherwise a part for the second kernel.  A
+// block has at most one run that begins inside a unit, and one that ends inside.
+template <typename T, int D, class Q>
+__device__ __forceinline__ void Finish(const CachedParams& p, Q& rows, int b, int head, int pair0, int lane, bool begins, bool ends, int runs,
+                                       int run, unsigned long long seen) {
+  rows.l += __shfl_xor(rows.l, 32);  // both halves of the wavefront hold the pair
+  if (begins && ends) {
+    const int pair = pair0 + (lane & 31), token = p.group(pair), group = p.group.value;
+    if (pair >= p.tokens * group) return;
+    char* out = const_cast<char*>(HeadOf<T>(p.o, b, head * group + pair - token * group)) + token * p.o.row * (int64_t)sizeof(T);
+    rows.Store(out, p.d, seen == 0 ? 0.0f : 1.0f / rows.l, lane >> 5);
+  } else {
+    if (seen == 0) rows.l = -1.0f;
+    rows.Hand(p.parts + ((int64_t)(2 * blockIdx.x + (begins ? 1 : 0)) * runs + run) * Q::kRegisters * 64, lane);
+  }
+}
+
 // D: d rounded up to an instance; WQ x 32 pairs per block, KG groups of wavefronts that take the tiles' keys in turn
 template <typename T, int D, int WQ, int KG>
 __global__ void __launch_bounds__(64 * WQ * KG)
 cached_attention_kernel(CachedParams p) {
   typedef Queries<T, D> Q;
-  typedef Layout<T, D> L;
+  typedef Padded<T, D> L;
   constexpr int THREADS = 64 * WQ * KG, KT = 32 * KG, NC = L::NC;
   constexpr int V_AT = KT * L::K_PITCH, HOLDS_AT = V_AT + KT * L::V_PITCH, STAGE = HOLDS_AT + KT;
   constexpr int MEET = (KG - 1) * WQ * 64 * Q::kRegisters * 4;
@@ -196,70 +213,475 @@ cached_attention_kernel(CachedParams p) {
       }
     }
     __syncthreads();  // the next unit's tiles may overwrite what was read here
-    if (kg == 0) {
-      // both halves of the wavefront hold this pair
-      rows.l += __shfl_xor(rows.l, 32);
-      if (tile0 == 0 && tile1 == tiles) {
-        if (pair0 + (lane & 31) < pairs) {
-          char* out = const_cast<char*>(HeadOf<T>(p.o, b, my_head)) + token * p.o.row * (int64_t)sizeof(T);
-          rows.Store(out, p.d, seen == 0 ? 0.0f : 1.0f / rows.l, half);
-        }
-      } else {
-        // a block has at most one run that begins inside a unit, and one that ends inside
-        if (seen == 0) rows.l = -1.0f;
-        rows.Hand(p.parts + ((int64_t)(2 * blockIdx.x + (tile0 == 0 ? 1 : 0)) * WQ + wq) * Q::kRegisters * 64, lane);
-      }
-    }
+    if (kg == 0) Finish<T, D>(p, rows, b, head, pair0, lane, tile0 == 0, tile1 == tiles, WQ, wq, seen);
     at += tile1 - tile0;
   }
 }
 
-// Units whose tiles several blocks had: a wavefront takes 4 of the 16 registers of each 32 elements of d, of 32 pairs.
-template <typename T, int D, int WQ, int KG>
+// zeros for the rows of keys that are none
+__device__ const u32x4 kZeros[32] = {};
+
+// 16 x PT pairs of a wavefront against 32 keys at a time, for units of few pairs: S^T = K Q^T by MFMAs of 16 keys x 16 pairs, a
+// lane holding the scores of pair lane % 16 (+ 16 per pair tile) for the keys 16 h + 4 (lane / 16) + r, which is, as it lies, the
+// second operand of O^T = V^T P^T.
+template <typename T, int D, int PT>
+struct FewPairs {
+  typedef Dense<T, D> L;
+  static constexpr bool F32 = L::F32;
+  static constexpr int STEPS = L::NC / 4, DT = D / 16;
+  u32x4 q[PT][STEPS];
+  float m[PT], l[PT];  // l: of this lane's keys only
+  f32x4 o[PT][DT];     // d = 16 t + 4 (lane / 16) + r
+
+  // the chunk of a row that a lane multiplies in step i: halves of a wavefront take neighbouring ones, whose place in LDS
+  // differs in the lowest bit
+  static __device__ __forceinline__ int ChunkOf(int i, int lane) { return 4 * i + 2 * ((lane >> 4) & 1) + (lane >> 5); }
+
+  __device__ __forceinline__ void Start(int tile, const char* row, int chunks, int lane, float scale) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      q[tile][i] = u32x4{0, 0, 0, 0};
+      if (ChunkOf(i, lane) < chunks) q[tile][i] = Signed<T>(LoadAny<T>(row + ChunkOf(i, lane) * 16), scale);
+    }
+    m[tile] = -__builtin_inff(), l[tile] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[tile][t] = f32x4{0, 0, 0, 0};
+  }
+  static __device__ __forceinline__ f32x4 Multiply(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (F32) {
+      const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+      return c;
+    } else {
+      typedef typename cinn_hip_kernels::flex::Half16<T> H;
+      return H::mfma(__builtin_bit_cast(typename H::vec8, a), __builtin_bit_cast(typename H::vec8, b), c);
+    }
+  }
+  __device__ __forceinline__ void Scores(f32x4 (&s)[PT][2], const char* tile, int lane) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int n = 0; n < PT; ++n) s[n][h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const u32x4 k = *reinterpret_cast<const u32x4*>(tile + L::At(16 * h + (lane & 15), ChunkOf(i, lane)));
+#pragma unroll
+        for (int n = 0; n < PT; ++n) s[n][h] = Multiply(k, q[n][i], s[n][h]);
+      }
+    }
+  }
+  static __device__ __forceinline__ void Mask(f32x4 (&s)[2], unsigned word, int lane) {
+    word >>= 4 * (lane >> 4);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (!((word >> (16 * h + r)) & 1)) s[h][r] = -__builtin_inff();
+  }
+  // as Queries::Soften
+  __device__ __forceinline__ void Soften(int tile, f32x4 (&s)[2], const Exp<T>& ex) {
+    float top = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e >> 2][e & 3]);
+    if (__ballot((top - m[tile]) * ex.c > 8.0f)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(m[tile], fmaxf(top, __shfl_xor(top, 32)));
+      const float keep = ex(m[tile], ex.Base(top));
+      l[tile] *= keep;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) o[tile][t] *= keep;
+      m[tile] = top;
+    }
+    const float base = ex.Base(m[tile]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      s[e >> 2][e & 3] = ex(s[e >> 2][e & 3], base);
+      l[tile] += s[e >> 2][e & 3];
+    }
+  }
+  // 16-bit probabilities round on their way into the matrix cores, as in Queries::Add
+  __device__ __forceinline__ void Add(const f32x4 (&s)[PT][2], const char* tile, int lane) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int key = 16 * (e >> 2) + 4 * (lane >> 4) + (e & 3);
+          const float v = *reinterpret_cast<const float*>(tile + L::At(key, 4 * t + ((lane & 15) >> 2)) + (lane & 3) * 4);
+#pragma unroll
+          for (int n = 0; n < PT; ++n) o[n][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[n][e >> 2][e & 3], o[n][t], 0, 0, 0);
+        }
+    } else {
+      typedef T vec8 __attribute__((ext_vector_type(8)));
+      vec8 pr[PT];
+#pragma unroll
+      for (int n = 0; n < PT; ++n)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pr[n][e] = (T)s[n][e >> 2][e & 3];
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        s16x4 part[2];  // four keys x sixteen d per group of 16 lanes, transposed on the way
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const char* at = tile + L::At(16 * h + 4 * (lane >> 4) + ((lane & 15) >> 2), 2 * t + ((lane & 3) >> 1)) + (lane & 1) * 8;
+          part[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)at);
+        }
+        const u32x4 v = __builtin_bit_cast(u32x4, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int n = 0; n < PT; ++n) o[n][t] = Multiply(v, __builtin_bit_cast(u32x4, pr[n]), o[n][t]);
+      }
+    }
+  }
+  // as Queries::Unbounded and Queries::AddChosen
+  static __device__ __forceinline__ bool Unbounded(const char* tile, int lane) {
+    constexpr unsigned kExponent = F32 ? 0x7f800000u : __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < L::NC / 2; ++i) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(tile + (i * 64 + lane) * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        found |= (v[e] & kExponent) == kExponent;
+        if (!F32) found |= (v[e] >> 16 & kExponent) == kExponent;
+      }
+    }
+    return __ballot(found) != 0;
+  }
+  __device__ __forceinline__ void AddChosen(const f32x4 (&s)[PT][2], const unsigned (&word)[PT], const char* tile, int lane) {
+#pragma unroll 1
+    for (int key = 0; key < 32; ++key) {
+      const int reg = (key >> 4) * 4 + (key & 3), owner = (key & 15) >> 2;
+#pragma unroll
+      for (int n = 0; n < PT; ++n) {
+        float prob = s[n][0][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) prob = reg == e ? s[n][e >> 2][e & 3] : prob;
+        prob = __shfl((float)(T)prob, owner * 16 + (lane & 15));
+        const bool chosen = (word[n] >> key) & 1;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int byte = (16 * t + 4 * (lane >> 4) + r) * (int)sizeof(T);
+            const float v  = (float)*reinterpret_cast<const T*>(tile + L::At(key, byte >> 4) + (byte & 15));
+            o[n][t][r]     = chosen ? __builtin_fmaf(prob, v, o[n][t][r]) : o[n][t][r];
+          }
+      }
+    }
+  }
+
+  // what another wavefront has of one pair tile, [register][lane]
+  static constexpr int kRegisters = DT * 4 + 2;
+  __device__ __forceinline__ void Hand(int tile, float* to, int lane) const {
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) to[(t * 4 + r) * 64 + lane] = o[tile][t][r];
+    to[(kRegisters - 2) * 64 + lane] = m[tile];
+    to[(kRegisters - 1) * 64 + lane] = l[tile];
+  }
+};
+
+// At most 16 PT pairs: a wavefront streams 32 keys of every tile through buffers of its own in LDS, STAGES deep for keys and
+// for values, that loads fill directly, and meets the others at the end of a unit only.  The next keys are requested as soon
+// as the scores are there, the next values when they are summed.  Which pages the rows lie in comes the same way, STAGES
+// tiles ahead of them: every wavefront's loads land in order, so that one count tells what has.
+template <typename T, int D, int PT, int WAVES, int STAGES>
+__global__ void __launch_bounds__(64 * WAVES, (WAVES + 3) / 4)
+cached_attention_few_kernel(CachedParams p) {
+  typedef FewPairs<T, D, PT> Q;
+  typedef Dense<T, D> L;
+  constexpr int KT = 32 * WAVES, NC = L::NC, N = NC / 2;  // N: loads for a tile of keys or of values
+  constexpr int RPL = 64 / NC;                            // rows per load, where that is a whole number
+  constexpr int IDS = 4 * STAGES, IDS_AT = STAGES * 2 * L::BYTES, ROWS_AT = IDS_AT + IDS * 256, WAVE = ROWS_AT + STAGES * 32 * 16;
+  constexpr int MEET = WAVES * PT * 64 * Q::kRegisters * 4;
+  __shared__ __attribute__((aligned(256))) char lds[WAVES * WAVE > MEET ? WAVES * WAVE : MEET];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int chunks = p.d * (int)sizeof(T) / 16, pairs = p.tokens * p.group.value;
+  const Exp<T> ex(p.scale);
+  char* mine = lds + wave * WAVE;
+  const unsigned mine_at = LdsAddress(mine);
+  // rows of whole loads in one page: a load has one base
+  const bool even_rows = L::POW2 && chunks == NC && p.page_rows.value % (L::POW2 ? RPL : 1) == 0;
+  const int row_bytes  = (int)(p.row * sizeof(T));
+  constexpr int TURNS  = NC == 32 ? 4 : NC == 16 ? 2 : 1;  // places of a row's chunks repeat with every TURNS loads
+  int lane_off[TURNS];
+#pragma unroll
+  for (int j = 0; j < TURNS; ++j) lane_off[j] = lane / NC * row_bytes + L::Back(lane % NC, L::RowTurn(j * RPL + lane / NC)) * 16;
+
+  int64_t at, end;  // this block's items
+  Place place;
+  if (p.blocks > 0) {
+    const int64_t total = Find(p, -1, KT).count, blocks = min((int64_t)p.blocks, total);
+    if (blockIdx.x >= blocks) return;
+    at = total * blockIdx.x / blocks, end = total * (blockIdx.x + 1) / blocks;
+    place = Find(p, at, KT);
+  } else {
+    const int b = blockIdx.x / p.units, length = LengthOf(p, b), tiles = (length + p.tokens + KT - 1) / KT;
+    at = (int64_t)(blockIdx.x % p.units) * tiles, end = at + tiles;
+    place = {b, length, 0, (int64_t)tiles * p.units};
+  }
+#pragma unroll 1
+  while (at < end) {
+    if (at >= place.first + place.count) place = Find(p, at, KT);
+    const int b = place.b, length = place.length, keys = length + p.tokens, tiles = (keys + KT - 1) / KT;
+    const int64_t inside = at - place.first;
+    const int head = (int)(inside / tiles), tile0 = (int)(inside - (int64_t)head * tiles);
+    const int tile1 = (int)min((int64_t)tiles, tile0 + end - at), last = tile1 - 1;
+    const char* k_new = HeadOf<T>(p.k, b, head);
+    const char* v_new = HeadOf<T>(p.v, b, head);
+    const int* table  = p.table + (int64_t)b * p.columns;
+
+    auto request_pages = [&](int kt) {
+      const int key = min(kt * KT + wave * 32 + (lane & 31), max(length - 1, 0));
+      CopyToLds4(table + p.page_rows(key), mine_at + IDS_AT + kt % IDS * 256);
+    };
+    // where a tile's rows lie: the offset in the pages of the lane's key's row, or with a key that is none or new among the 32
+    // the rows' addresses in LDS
+    int64_t off[STAGES];
+    unsigned holds[STAGES];  // which of the 32 keys are some
+    bool plain[STAGES];
+    struct Two { const char *k, *v; };
+    auto place_rows = [&](int kt, int stage) {
+      const int key = kt * KT + wave * 32 + (lane & 31);
+      const int page = *reinterpret_cast<const int*>(mine + IDS_AT + kt % IDS * 256 + (lane & 31) * 4);
+      const bool good = key < length && page >= 0 && page < p.pages;
+      const int64_t offset = good ? (page * p.page + (key - p.page_rows(key) * p.page_rows.value) * p.row + head * p.head) * (int64_t)sizeof(T) : 0;
+      const unsigned word = (unsigned)__ballot(good || (key >= length && key < keys));
+      const bool straight = even_rows && __ballot(good) == ~0ull;
+#pragma unroll
+      for (int s = 0; s < STAGES; ++s)
+        if (stage == s) off[s] = offset, holds[s] = word, plain[s] = straight;
+      if (!straight) {
+        Two row = {reinterpret_cast<const char*>(kZeros), reinterpret_cast<const char*>(kZeros)};
+        if (good) row = {p.k_pages + offset, p.v_pages + offset};
+        if (key >= length && key < keys)
+          row = {k_new + (key - length) * p.k.row * (int64_t)sizeof(T), v_new + (key - length) * p.v.row * (int64_t)sizeof(T)};
+        if (lane < 32) reinterpret_cast<Two*>(mine + ROWS_AT)[stage * 32 + lane] = row;
+      }
+    };
+    auto request = [&](int stage, bool values) {
+      const unsigned to = mine_at + (2 * stage + values) * L::BYTES;
+      bool straight = plain[0];
+      int64_t offset = off[0];
+#pragma unroll
+      for (int s = 1; s < STAGES; ++s)
+        if (stage == s) straight = plain[s], offset = off[s];
+      if (straight) {
+        const char* pages = values ? p.v_pages : p.k_pages;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const unsigned low = __builtin_amdgcn_readlane((unsigned)offset, j * RPL % 32);
+          const unsigned high = __builtin_amdgcn_readlane((unsigned)(offset >> 32), j * RPL % 32);
+          CopyToLds16(pages + (int64_t)((uint64_t)high << 32 | low), (unsigned)lane_off[j % TURNS], to + j * 1024);
+        }
+      } else {
+        const Two* rows = reinterpret_cast<const Two*>(mine + ROWS_AT) + stage * 32;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const int slot = j * 64 + lane, row = slot / NC, c = L::Back(slot % NC, L::RowTurn(row));
+          const char* from = values ? rows[row].v : rows[row].k;
+          CopyToLds16(c < chunks ? from + c * 16 : reinterpret_cast<const char*>(kZeros), to + j * 1024);
+        }
+      }
+    };
+
+    Q rows;
+    unsigned long long seen[PT];
+#pragma unroll
+    for (int n = 0; n < PT; ++n) {
+      const int pair = min(n * 16 + (lane & 15), pairs - 1), token = p.group(pair), my_head = head * p.group.value + pair - token * p.group.value;
+      rows.Start(n, HeadOf<T>(p.q, b, my_head) + token * p.q.row * (int64_t)sizeof(T), chunks, lane, p.scale);
+      seen[n] = SeenBy(p, b, token);
+    }
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) request_pages(min(tile0 + i, last));
+    WaitForAllBut<0>();
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) {
+      if (tile0 + i > last) break;
+      request_pages(min(tile0 + STAGES + i, last));
+      place_rows(tile0 + i, i);
+      request(i, false);
+      request(i, true);
+    }
+    int stage = 0;
+#pragma unroll 1
+    for (int kt = tile0; kt < tile1; ++kt) {
+      const bool more = kt + STAGES <= last;
+      const int behind = min(last - kt, STAGES - 1);  // tiles that are on their way behind this one
+      const char* cur = mine + stage * 2 * L::BYTES;
+      if (STAGES > 1 && behind == 1) {
+        WaitForAllBut<N + (STAGES > 1 ? 1 : 0) * (2 * N + 1)>();
+      } else if (STAGES > 2 && behind == 2) {
+        WaitForAllBut<N + (STAGES > 2 ? 2 : 0) * (2 * N + 1)>();
+      } else if (STAGES > 3 && behind == 3) {
+        WaitForAllBut<N + (STAGES > 3 ? 3 : 0) * (2 * N + 1)>();
+      } else {
+        WaitForAllBut<N>();
+      }
+      asm volatile("" ::: "memory");
+      f32x4 s[PT][2];
+      rows.Scores(s, cur, lane);
+      unsigned some = holds[0];
+#pragma unroll
+      for (int n = 1; n < STAGES; ++n) some = stage == n ? holds[n] : some;
+      if (more) {
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // the keys have been read
+        request_pages(min(kt + 2 * STAGES, last));
+        place_rows(kt + STAGES, stage);
+        request(stage, false);
+      }
+      const int j0 = kt * KT + wave * 32 - length;
+      unsigned word[PT];
+      bool masked = false;
+#pragma unroll
+      for (int n = 0; n < PT; ++n) {
+        word[n] = some & (j0 >= 0 ? j0 < 64 ? (unsigned)(seen[n] >> j0) : 0u : j0 <= -32 ? ~0u : (unsigned)(seen[n] << -j0) | Below(-j0));
+        if (seen[n] == 0) word[n] = 0;
+        masked |= __ballot(word[n] != ~0u) != 0;
+      }
+#pragma unroll
+      for (int n = 0; n < PT; ++n) {
+        if (masked) Q::Mask(s[n], word[n], lane);
+        rows.Soften(n, s[n], ex);
+      }
+      if (more) {
+        if (STAGES > 1 && behind == 1) {
+          WaitForAllBut<N + 1 + (STAGES > 1 ? 1 : 0) * (2 * N + 1)>();
+        } else if (STAGES > 2 && behind == 2) {
+          WaitForAllBut<N + 1 + (STAGES > 2 ? 2 : 0) * (2 * N + 1)>();
+        } else if (STAGES > 3 && behind == 3) {
+          WaitForAllBut<N + 1 + (STAGES > 3 ? 3 : 0) * (2 * N + 1)>();
+        } else {
+          WaitForAllBut<N + 1>();
+        }
+      } else if (STAGES > 1 && behind == 1) {
+        WaitForAllBut<(STAGES > 1 ? 1 : 0) * (2 * N + 1)>();
+      } else if (STAGES > 2 && behind == 2) {
+        WaitForAllBut<(STAGES > 2 ? 2 : 0) * (2 * N + 1)>();
+      } else if (STAGES > 3 && behind == 3) {
+        WaitForAllBut<(STAGES > 3 ? 3 : 0) * (2 * N + 1)>();
+      } else {
+        WaitForAllBut<0>();
+      }
+      asm volatile("" ::: "memory");
+      if (masked && Q::Unbounded(cur + L::BYTES, lane)) {
+        rows.AddChosen(s, word, cur + L::BYTES, lane);
+      } else {
+        rows.Add(s, cur + L::BYTES, lane);
+      }
+      if (more) {
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // the values have been read
+        request(stage, true);
+      }
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+    }
+    // the wavefronts' sums of the same pairs: each adds up a share of them
+    __syncthreads();
+    float* meet = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int n = 0; n < PT; ++n) {
+      rows.l[n] += __shfl_xor(rows.l[n], 16);
+      rows.l[n] += __shfl_xor(rows.l[n], 32);
+      rows.Hand(n, meet + (wave * PT + n) * Q::kRegisters * 64, lane);
+    }
+    __syncthreads();
+    const bool whole = tile0 == 0 && tile1 == tiles;
+#pragma unroll
+    for (int n = 0; n < PT; ++n) {
+      const float* from = meet + n * Q::kRegisters * 64 + lane;
+      constexpr int EACH = PT * Q::kRegisters * 64;
+      float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) top = fmaxf(top, from[w * EACH + (Q::kRegisters - 2) * 64]);
+      const float base = ex.Base(top);
+      float f[WAVES];
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        f[w] = ex(from[w * EACH + (Q::kRegisters - 2) * 64], base);
+        sum  = __builtin_fmaf(from[w * EACH + (Q::kRegisters - 1) * 64], f[w], sum);
+      }
+      const int pair = n * 16 + (lane & 15), token = p.group(min(pair, pairs - 1));
+      const int my_head = head * p.group.value + min(pair, pairs - 1) - token * p.group.value;
+      char* out = const_cast<char*>(HeadOf<T>(p.o, b, my_head)) + token * p.o.row * (int64_t)sizeof(T);
+      float* part = p.parts + ((int64_t)(2 * blockIdx.x + (tile0 == 0 ? 1 : 0)) * PT + n) * Q::kRegisters * 64 + lane;
+      for (int t = wave; t < Q::DT; t += WAVES) {
+        float four[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          four[r] = 0.0f;
+#pragma unroll
+          for (int w = 0; w < WAVES; ++w) four[r] = __builtin_fmaf(from[w * EACH + (t * 4 + r) * 64], f[w], four[r]);
+        }
+        if (whole) {
+          const int to = 16 * t + 4 * (lane >> 4);
+          T rounded[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) rounded[r] = (T)(seen[n] == 0 ? 0.0f : four[r] / sum);
+          if (pair < pairs && to < p.d) __builtin_memcpy(out + to * sizeof(T), rounded, sizeof(rounded));
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) part[(t * 4 + r) * 64] = four[r];
+        }
+      }
+      if (!whole && wave == 0) {
+        part[(Q::kRegisters - 2) * 64] = top;
+        part[(Q::kRegisters - 1) * 64] = seen[n] == 0 ? -1.0f : sum;
+      }
+    }
+    __syncthreads();  // the next unit's tiles may overwrite what was read here
+    at += tile1 - tile0;
+  }
+}
+
+// Units whose tiles several blocks had: a wavefront takes four registers of the lanes of TILE pairs, four consecutive elements
+// of d.  RUNS: of TILE pairs in a block's unit.
+template <typename T, int D, int TILE, int RUNS>
 __global__ void __launch_bounds__(64)
-cached_attention_join_kernel(CachedParams p) {
-  typedef Queries<T, D> Q;
-  typedef Layout<T, D> L;
-  constexpr int KT = 32 * KG, QUARTERS = L::DT * 4;
-  const int lane = threadIdx.x, quarter = blockIdx.x % QUARTERS, wq = blockIdx.x / QUARTERS % WQ, which = blockIdx.x / QUARTERS / WQ;
+cached_attention_join_kernel(CachedParams p, int keys_per_tile) {
+  constexpr int GROUPS = 64 / TILE, QUADS = D / 4 / GROUPS, REGISTERS = QUADS * 4 + 2;  // lanes of one pair, fours of registers
+  const int lane = threadIdx.x, quad = blockIdx.x % QUADS, run = blockIdx.x / QUADS % RUNS, which = blockIdx.x / QUADS / RUNS;
   const int b = which / p.units, unit = which % p.units, pairs = p.tokens * p.group.value;
-  const int pair = (unit / p.kv_heads * WQ + wq) * 32 + (lane & 31);
-  if ((unit / p.kv_heads * WQ + wq) * 32 >= pairs || quarter * 8 >= p.d) return;
+  const int pair0 = (unit / p.kv_heads * RUNS + run) * TILE, pair = pair0 + lane % TILE;
+  if (pair0 >= pairs || quad * 4 * GROUPS >= p.d) return;
   int64_t total = 0, first = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
     int64_t mine = 0;
-    if (b0 + lane < p.batch) mine = (int64_t)((LengthOf(p, b0 + lane) + p.tokens + KT - 1) / KT) * p.units;
+    if (b0 + lane < p.batch) mine = (int64_t)((LengthOf(p, b0 + lane) + p.tokens + keys_per_tile - 1) / keys_per_tile) * p.units;
     int64_t before = b0 + lane < b ? mine : 0;
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) mine += __shfl_xor((long long)mine, x), before += __shfl_xor((long long)before, x);
     total += mine, first += before;
   }
-  const int tiles = (LengthOf(p, b) + p.tokens + KT - 1) / KT;
+  const int tiles = (LengthOf(p, b) + p.tokens + keys_per_tile - 1) / keys_per_tile;
   first += (int64_t)unit * tiles;
   const int64_t blocks = min((int64_t)p.blocks, total);
   const int block0 = (int)(((first + 1) * blocks - 1) / total), block1 = (int)(((first + tiles) * blocks - 1) / total);
   if (block0 == block1) return;  // that block has written the result
   auto part = [&](int block) {
-    return p.parts + ((int64_t)(2 * block + (block == block0 ? 1 : 0)) * WQ + wq) * Q::kRegisters * 64 + lane;
+    return p.parts + ((int64_t)(2 * block + (block == block0 ? 1 : 0)) * RUNS + run) * REGISTERS * 64 + lane;
   };
   const Exp<T> ex(p.scale);
   float top = -__builtin_inff();
 #pragma unroll 4
-  for (int i = block0; i <= block1; ++i) top = fmaxf(top, part(i)[(Q::kRegisters - 2) * 64]);
+  for (int i = block0; i <= block1; ++i) top = fmaxf(top, part(i)[(REGISTERS - 2) * 64]);
   const float base = ex.Base(top);
   float sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
   for (int i = block0; i <= block1; ++i) {
     const float* from = part(i);
-    const float f     = ex(from[(Q::kRegisters - 2) * 64], base);
-    sum               = __builtin_fmaf(from[(Q::kRegisters - 1) * 64], f, sum);
+    const float f     = ex(from[(REGISTERS - 2) * 64], base);
+    sum               = __builtin_fmaf(from[(REGISTERS - 1) * 64], f, sum);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(from[(quarter * 4 + e) * 64], f, o[e]);
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(from[(quad * 4 + e) * 64], f, o[e]);
   }
-  const bool token_is_none = part(block0)[(Q::kRegisters - 1) * 64] < 0.0f;
+  const bool token_is_none = part(block0)[(REGISTERS - 1) * 64] < 0.0f;
   if (pair >= pairs) return;
   const int token = p.group(pair), my_head = unit % p.kv_heads * p.group.value + pair - token * p.group.value;
-  const int at = quarter / 4 * 32 + quarter % 4 * 8 + 4 * (lane >> 5);
+  const int at = (quad * GROUPS + lane / TILE) * 4;
   T four[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) four[e] = (T)(token_is_none ? 0.0f : o[e] / sum);
@@ -267,34 +689,54 @@ cached_attention_join_kernel(CachedParams p) {
   if (at < p.d) __builtin_memcpy(out, four, sizeof(four));
 }
 
-template <typename T, int D, int WQ, int KG>
-void LaunchBlocks(CachedParams p, hipStream_t stream) {
-  constexpr int KT = 32 * KG, kMostBlocks = 256;
+// Blocks that divide the list of tiles of `keys_per_tile` keys, or one per unit of `runs` x `tile` pairs.
+template <int D>
+int Divide(CachedParams& p, int tile, int runs, int keys_per_tile, hipStream_t stream) {
+  constexpr int kMostBlocks = 256;
   const int pairs  = p.tokens * p.group.value;
-  p.units          = p.kv_heads * ((pairs + 32 * WQ - 1) / (32 * WQ));
+  p.units          = p.kv_heads * ((pairs + tile * runs - 1) / (tile * runs));
   const int units  = p.batch * p.units;
-  const int64_t most_tiles = ((int64_t)p.columns * p.page_rows.value + p.tokens + KT - 1) / KT;
+  const int64_t most_tiles = ((int64_t)p.columns * p.page_rows.value + p.tokens + keys_per_tile - 1) / keys_per_tile;
   p.blocks = 0;
   if (most_tiles > 4) {
     const int blocks   = (int)std::min<int64_t>(kMostBlocks, units * most_tiles);
-    const size_t bytes = (size_t)2 * blocks * WQ * Queries<T, D>::kRegisters * 64 * sizeof(float);
+    const size_t bytes = (size_t)2 * blocks * runs * (D * tile / 64 + 2) * 64 * sizeof(float);
     if (bytes <= cinn_hip_kernels::ScratchLimit(cinn_hip_kernels::ScratchKind::kSplitK, stream)) {
       p.blocks = blocks;
       p.parts  = static_cast<float*>(cinn_hip_kernels::Scratch(cinn_hip_kernels::ScratchKind::kSplitK, bytes, stream));
     }
   }
-  hipLaunchKernelGGL((cached_attention_kernel<T, D, WQ, KG>), dim3((unsigned)(p.blocks > 0 ? p.blocks : units)), dim3(64 * WQ * KG), 0, stream, p);
-  if (p.blocks > 0)
-    hipLaunchKernelGGL((cached_attention_join_kernel<T, D, WQ, KG>), dim3((unsigned)(units * WQ * Layout<T, D>::DT * 4)), dim3(64), 0, stream, p);
+  return p.blocks > 0 ? p.blocks : units;
+}
+
+template <typename T, int D, int TILE, int RUNS>
+void LaunchJoin(const CachedParams& p, int keys_per_tile, hipStream_t stream) {
+  if (p.blocks == 0) return;
+  hipLaunchKernelGGL((cached_attention_join_kernel<T, D, TILE, RUNS>), dim3((unsigned)(p.batch * p.units * RUNS * (D * TILE / 256))), dim3(64), 0,
+                     stream, p, keys_per_tile);
+}
+
+template <typename T, int D, int PT>
+void LaunchFew(CachedParams p, hipStream_t stream) {
+  // the buffers of eight (fp32 of more than 64 elements: four) wavefronts in 128 KiB of LDS
+  constexpr int kTile = 2 * Dense<T, D>::BYTES, kWaves = kTile > 16384 ? 4 : 8, kDeep = 128 * 1024 / kWaves / kTile;
+  constexpr int kStages = kDeep > 2 ? 2 : kDeep;
+  const int blocks = Divide<D>(p, 16, PT, 32 * kWaves, stream);
+  hipLaunchKernelGGL((cached_attention_few_kernel<T, D, PT, kWaves, kStages>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream, p);
+  LaunchJoin<T, D, 16, PT>(p, 32 * kWaves, stream);
 }
 
 template <typename T, int D>
-void LaunchTiles(const CachedParams& p, hipStream_t stream) {
+void LaunchTiles(CachedParams p, hipStream_t stream) {
   const int pairs = p.tokens * p.group.value;
-  if (pairs <= 32) {
-    LaunchBlocks<T, D, 1, sizeof(T) == 4 ? 2 : 4>(p, stream);
+  if (pairs <= 16) {
+    LaunchFew<T, D, 1>(p, stream);
+  } else if (pairs <= 32) {
+    LaunchFew<T, D, 2>(p, stream);
   } else {
-    LaunchBlocks<T, D, 4, 2>(p, stream);
+    const int blocks = Divide<D>(p, 32, 4, 64, stream);
+    hipLaunchKernelGGL((cached_attention_kernel<T, D, 4, 2>), dim3((unsigned)blocks), dim3(512), 0, stream, p);
+    LaunchJoin<T, D, 32, 4>(p, 64, stream);
   }
 }
 

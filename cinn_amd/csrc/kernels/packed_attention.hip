@@ -80,7 +80,7 @@ template <typename T, int D, int WQ, int KG>
 __global__ void __launch_bounds__(64 * WQ * KG, 2)
 packed_attention_kernel(PackedParams p) {
   typedef Queries<T, D> Q;
-  typedef Layout<T, D> L;
+  typedef Padded<T, D> L;
   constexpr int THREADS = 64 * WQ * KG, KT = 32 * KG, NC = L::NC;
   constexpr int V_AT = KT * L::K_PITCH, STAGE = V_AT + KT * L::V_PITCH;
   constexpr int MEET = (KG - 1) * WQ * 64 * Q::kRegisters * 4;
