@@ -42,6 +42,10 @@ __device__ __forceinline__ int LengthOf(const CachedParams& p, int b) {
   return min(max(p.lengths[b], 0), p.columns * p.page_rows.value);
 }
 
+// What a block's change of units costs beside its tiles, in tiles: every unit has that many empty items in front, so that the
+// blocks with many short sequences have fewer of them.
+constexpr int kEmpty = 1;
+
 // Where item `item` of the list of all tiles lies: its sequence, that one's rows in the cache and first item.  With item < 0
 // only the items are counted.  By every wavefront for itself, 64 sequences at a time.
 struct Place {
@@ -53,7 +57,7 @@ __device__ __forceinline__ Place Find(const CachedParams& p, int64_t item, int k
   int64_t before = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
     const int length = b0 + lane < p.batch ? LengthOf(p, b0 + lane) : 0;
-    const int64_t mine = b0 + lane < p.batch ? (int64_t)((length + p.tokens + keys_per_tile - 1) / keys_per_tile) * p.units : 0;
+    const int64_t mine = b0 + lane < p.batch ? (int64_t)((length + p.tokens + keys_per_tile - 1) / keys_per_tile + kEmpty) * p.units : 0;
     int64_t sum = mine;
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) {
@@ -129,16 +133,18 @@ cached_attention_kernel(CachedParams p) {
     place = Find(p, at, KT);
   } else {
     const int b = blockIdx.x / p.units, length = LengthOf(p, b), tiles = (length + p.tokens + KT - 1) / KT;
-    at = (int64_t)(blockIdx.x % p.units) * tiles, end = at + tiles;
-    place = {b, length, 0, (int64_t)tiles * p.units};
+    at = (int64_t)(blockIdx.x % p.units) * (tiles + kEmpty), end = at + tiles + kEmpty;
+    place = {b, length, 0, (int64_t)(tiles + kEmpty) * p.units};
   }
 #pragma unroll 1
   while (at < end) {
     if (at >= place.first + place.count) place = Find(p, at, KT);
     const int b = place.b, length = place.length, keys = length + p.tokens, tiles = (keys + KT - 1) / KT;
-    const int64_t inside = at - place.first;
-    const int unit = (int)(inside / tiles), tile0 = (int)(inside - (int64_t)unit * tiles);
-    const int tile1 = (int)min((int64_t)tiles, tile0 + end - at);
+    const int64_t inside = at - place.first, items = tiles + kEmpty;
+    const int unit = (int)(inside / items), item0 = (int)(inside - unit * items), item1 = (int)min(items, item0 + end - at);
+    const int tile0 = max(item0 - kEmpty, 0), tile1 = item1 - kEmpty;
+    at += item1 - item0;
+    if (tile0 >= tile1) continue;
     const int head = unit % p.kv_heads, pair0 = (unit / p.kv_heads * WQ + wq) * 32;
     const int pair = min(pair0 + (lane & 31), pairs - 1), token = p.group(pair), my_head = head * p.group.value + pair - token * p.group.value;
     const unsigned long long seen = SeenBy(p, b, token);
@@ -214,7 +220,6 @@ cached_attention_kernel(CachedParams p) {
     }
     __syncthreads();  // the next unit's tiles may overwrite what was read here
     if (kg == 0) Finish<T, D>(p, rows, b, head, pair0, lane, tile0 == 0, tile1 == tiles, WQ, wq, seen);
-    at += tile1 - tile0;
   }
 }
 
@@ -420,16 +425,18 @@ cached_attention_few_kernel(CachedParams p) {
     place = Find(p, at, KT);
   } else {
     const int b = blockIdx.x / p.units, length = LengthOf(p, b), tiles = (length + p.tokens + KT - 1) / KT;
-    at = (int64_t)(blockIdx.x % p.units) * tiles, end = at + tiles;
-    place = {b, length, 0, (int64_t)tiles * p.units};
+    at = (int64_t)(blockIdx.x % p.units) * (tiles + kEmpty), end = at + tiles + kEmpty;
+    place = {b, length, 0, (int64_t)(tiles + kEmpty) * p.units};
   }
 #pragma unroll 1
   while (at < end) {
     if (at >= place.first + place.count) place = Find(p, at, KT);
     const int b = place.b, length = place.length, keys = length + p.tokens, tiles = (keys + KT - 1) / KT;
-    const int64_t inside = at - place.first;
-    const int head = (int)(inside / tiles), tile0 = (int)(inside - (int64_t)head * tiles);
-    const int tile1 = (int)min((int64_t)tiles, tile0 + end - at), last = tile1 - 1;
+    const int64_t inside = at - place.first, items = tiles + kEmpty;
+    const int head = (int)(inside / items), item0 = (int)(inside - head * items), item1 = (int)min(items, item0 + end - at);
+    const int tile0 = max(item0 - kEmpty, 0), tile1 = item1 - kEmpty, last = tile1 - 1;
+    at += item1 - item0;
+    if (tile0 >= tile1) continue;
     const char* k_new = HeadOf<T>(p.k, b, head);
     const char* v_new = HeadOf<T>(p.v, b, head);
     const int* table  = p.table + (int64_t)b * p.columns;
@@ -633,7 +640,6 @@ cached_attention_few_kernel(CachedParams p) {
       }
     }
     __syncthreads();  // the next unit's tiles may overwrite what was read here
-    at += tile1 - tile0;
   }
 }
 
@@ -650,14 +656,14 @@ cached_attention_join_kernel(CachedParams p, int keys_per_tile) {
   int64_t total = 0, first = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
     int64_t mine = 0;
-    if (b0 + lane < p.batch) mine = (int64_t)((LengthOf(p, b0 + lane) + p.tokens + keys_per_tile - 1) / keys_per_tile) * p.units;
+    if (b0 + lane < p.batch) mine = (int64_t)((LengthOf(p, b0 + lane) + p.tokens + keys_per_tile - 1) / keys_per_tile + kEmpty) * p.units;
     int64_t before = b0 + lane < b ? mine : 0;
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) mine += __shfl_xor((long long)mine, x), before += __shfl_xor((long long)before, x);
     total += mine, first += before;
   }
   const int tiles = (LengthOf(p, b) + p.tokens + keys_per_tile - 1) / keys_per_tile;
-  first += (int64_t)unit * tiles;
+  first += (int64_t)unit * (tiles + kEmpty) + kEmpty;
   const int64_t blocks = min((int64_t)p.blocks, total);
   const int block0 = (int)(((first + 1) * blocks - 1) / total), block1 = (int)(((first + tiles) * blocks - 1) / total);
   if (block0 == block1) return;  // that block has written the result
