@@ -113,7 +113,14 @@ struct Dense : Shape<T, D> {
   static __device__ __forceinline__ int RowTurn(int row) {
     return NC % 16 == 0 ? 2 * (row & 7) : NC % 8 == 0 ? 2 * ((row >> 1) & 3) : 2 * ((row >> 2) & 1);
   }
-  static __device__ __forceinline__ int At(int row, int c) { return (row * NC + Turn(c, RowTurn(row))) * 16; }
+  // four rows' 64 bytes, which a transposing read of 32 columns takes together, in different quarters; single floats: the
+  // halves for rows four apart
+  static __device__ __forceinline__ int WideTurn(int row) {
+    if (F32) return NC > 8 ? 8 * ((row >> 2) & 1) : 0;
+    return NC == 16 ? 4 * (row & 3) : NC == 8 ? 4 * ((row >> 1) & 1) : 0;
+  }
+  static __device__ __forceinline__ int KAt(int row, int c) { return (row * NC + Turn(c, RowTurn(row))) * 16; }
+  static __device__ __forceinline__ int VAt(int row, int c) { return (row * NC + Turn(c, WideTurn(row))) * 16; }
 };
 
 // the bits of a word of 32 keys below `count`
@@ -160,13 +167,16 @@ struct Queries {
       if (!((word >> (8 * (r >> 2) + (r & 3))) & 1)) s[r] = -__builtin_inff();
   }
 
-  // scores -> probabilities against the running maximum; what has been summed is rescaled only when a score exceeds it by
+  // Scores become probabilities against a running maximum.  What has been summed is rescaled only when a score exceeds it by
   // more than a factor of 2^8 (fp32, whose exponent is natural: e^8), and only then do the lanes of a query agree on a new
-  // one: probabilities up to 256 (2981) lose nothing in either type, and after the first tiles few maxima grow that much
-  __device__ __forceinline__ void Soften(f32x16& s, const Exp<T>& ex) {
+  // one: probabilities up to 256 (2981) lose nothing in either type, and after the first tiles few maxima grow that much.
+  static __device__ __forceinline__ float Top(const f32x16& s) {
     float top = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+    return top;
+  }
+  __device__ __forceinline__ void Grow(float top, const Exp<T>& ex) {
     if (__ballot((top - m) * ex.c > 8.0f)) {
       top = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
       const float keep = ex(m, ex.Base(top));
@@ -177,6 +187,8 @@ struct Queries {
         for (int r = 0; r < 16; ++r) o[t][r] *= keep;
       m = top;
     }
+  }
+  __device__ __forceinline__ void Soften(f32x16& s, const Exp<T>& ex) {
     const float base = ex.Base(m);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -267,6 +279,7 @@ struct Queries {
     f32x16 s = Scores(k_tile, lane);
     const bool masked = __ballot(word != ~0u) != 0;
     if (masked) Mask(s, word, lane);
+    Grow(Top(s), ex);
     Soften(s, ex);
     if (masked && Unbounded(v_tile, chunks, lane)) {
       AddChosen(s, word, v_tile, lane);
@@ -323,6 +336,9 @@ struct Divisor {
   __device__ __forceinline__ int operator()(int v) const { return (int)((uint64_t)(unsigned)v * multiplier >> (31 + shift)); }
 };
 
+// zeros for rows and chunks that are none
+__device__ const u32x4 kZeros[32] = {};
+
 // Loads from memory straight to LDS: 16 bytes (4 bytes) a lane, written at LDS address `to` + 16 (4) * lane.  Inline assembly,
 // so that the compiler does not track them: tracked, it would wait for all of them before every LDS read.
 __device__ __forceinline__ void CopyToLds16(const void* from, unsigned to) {
@@ -332,6 +348,9 @@ __device__ __forceinline__ void CopyToLds16(const void* from, unsigned to) {
 // from a base that the wavefront shares and a lane's offset
 __device__ __forceinline__ void CopyToLds16(const void* base, unsigned off, unsigned to) {
   to = __builtin_amdgcn_readfirstlane(to);
+  const uint64_t at = (uint64_t)base;
+  base = (const void*)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(at >> 32)) << 32 |
+                       (unsigned)__builtin_amdgcn_readfirstlane((unsigned)at));
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(off), "s"(base) : "memory");
 }
 __device__ __forceinline__ void CopyToLds4(const void* from, unsigned to) {

@@ -223,9 +223,6 @@ cached_attention_kernel(CachedParams p) {
   }
 }
 
-// zeros for the rows of keys that are none
-__device__ const u32x4 kZeros[32] = {};
-
 // 16 x PT pairs of a wavefront against 32 keys at a time, for units of few pairs: S^T = K Q^T by MFMAs of 16 keys x 16 pairs, a
 // lane holding the scores of pair lane % 16 (+ 16 per pair tile) for the keys 16 h + 4 (lane / 16) + r, which is, as it lies, the
 // second operand of O^T = V^T P^T.
@@ -270,7 +267,7 @@ struct FewPairs {
       for (int n = 0; n < PT; ++n) s[n][h] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
-        const u32x4 k = *reinterpret_cast<const u32x4*>(tile + L::At(16 * h + (lane & 15), ChunkOf(i, lane)));
+        const u32x4 k = *reinterpret_cast<const u32x4*>(tile + L::KAt(16 * h + (lane & 15), ChunkOf(i, lane)));
 #pragma unroll
         for (int n = 0; n < PT; ++n) s[n][h] = Multiply(k, q[n][i], s[n][h]);
       }
@@ -313,7 +310,7 @@ struct FewPairs {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int key = 16 * (e >> 2) + 4 * (lane >> 4) + (e & 3);
-          const float v = *reinterpret_cast<const float*>(tile + L::At(key, 4 * t + ((lane & 15) >> 2)) + (lane & 3) * 4);
+          const float v = *reinterpret_cast<const float*>(tile + L::KAt(key, 4 * t + ((lane & 15) >> 2)) + (lane & 3) * 4);
 #pragma unroll
           for (int n = 0; n < PT; ++n) o[n][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[n][e >> 2][e & 3], o[n][t], 0, 0, 0);
         }
@@ -329,7 +326,7 @@ struct FewPairs {
         s16x4 part[2];  // four keys x sixteen d per group of 16 lanes, transposed on the way
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const char* at = tile + L::At(16 * h + 4 * (lane >> 4) + ((lane & 15) >> 2), 2 * t + ((lane & 3) >> 1)) + (lane & 1) * 8;
+          const char* at = tile + L::KAt(16 * h + 4 * (lane >> 4) + ((lane & 15) >> 2), 2 * t + ((lane & 3) >> 1)) + (lane & 1) * 8;
           part[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)at);
         }
         const u32x4 v = __builtin_bit_cast(u32x4, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
@@ -369,7 +366,7 @@ struct FewPairs {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int byte = (16 * t + 4 * (lane >> 4) + r) * (int)sizeof(T);
-            const float v  = (float)*reinterpret_cast<const T*>(tile + L::At(key, byte >> 4) + (byte & 15));
+            const float v  = (float)*reinterpret_cast<const T*>(tile + L::KAt(key, byte >> 4) + (byte & 15));
             o[n][t][r]     = chosen ? __builtin_fmaf(prob, v, o[n][t][r]) : o[n][t][r];
           }
       }

@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <climits>
 #include <cstdint>
+#include <cstdlib>
 
 #include "cinn_hip_runtime.h"
 #include "kernels/attention_tile.h"
@@ -53,10 +54,10 @@ __device__ __forceinline__ Found Find(const PackedParams& p, int tile, int tile_
     const unsigned long long behind = __ballot(before + sum > tile);
     if (behind) {
       const int at = __ffsll(behind) - 1;
-      const int all = __shfl(tiles, at), here = tile - (before + __shfl(sum, at) - all);
-      return {__shfl(first, at), __shfl(count, at), all - 1 - here, 0};  // the longest first
+      const int all = __builtin_amdgcn_readlane(tiles, at), here = tile - (before + __builtin_amdgcn_readlane(sum, at) - all);
+      return {__builtin_amdgcn_readlane(first, at), __builtin_amdgcn_readlane(count, at), all - 1 - here, 0};  // the longest first
     }
-    before += __shfl(sum, 63);
+    before += __builtin_amdgcn_readlane(sum, 63);
   }
   return {0, 0, tile - before, p.tiles - before};
 }
@@ -167,14 +168,162 @@ packed_attention_kernel(PackedParams p) {
   rows.Store(out, p.d, 1.0f / sum, half);
 }
 
+// 16-bit types: WQ wavefronts of 32 pairs, tiles of 32 STEPS keys in a ring of four in LDS that loads fill directly, one
+// barrier per tile.  A wavefront multiplies the next 32 keys by its queries while it takes the exponentials of the last
+// scores: the matrix cores and the vector unit work side by side, within a wavefront and, two of them to a SIMD, across.
+// Rows behind the last key are rows of the tensor all the same; nothing attends to them.
+template <typename T, int D, int WQ, int STEPS>
+__global__ void __launch_bounds__(64 * WQ, 2)
+packed_attention_ring_kernel(PackedParams p) {
+  typedef Dense<T, D> L;
+  typedef Queries<T, D, L> Q;
+  constexpr int KT = 32 * STEPS, NC = L::NC, STAGE = 2 * STEPS * L::BYTES, STAGES = 4;
+  constexpr int N  = STEPS * NC / WQ;  // loads of a wavefront for a tile, whose values lie behind its keys
+  static_assert(N * WQ == STEPS * NC && STAGES * STAGE <= 160 * 1024 && 2 * N < 64);
+  __shared__ __attribute__((aligned(256))) char lds[STAGES * STAGE];
+
+  const int head = blockIdx.x % p.kv_heads;
+  const Found at = Find(p, blockIdx.x / p.kv_heads, 32 * WQ);
+  if (at.count == 0) {
+    ClearRest<T>(p, head, at.tile, at.more);
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int chunks = p.d * (int)sizeof(T) / 16, pairs = at.count * p.group.value;
+  const int pair0 = (at.tile * WQ + wave) * 32;
+  const int pair = min(pair0 + (lane & 31), pairs - 1);
+  const int query = p.group(pair), my_head = head * p.group.value + pair - query * p.group.value;
+  const int first_query = p.group(min(pair0, pairs - 1)), last_query = pair0 < pairs ? p.group(min(pair0 + 31, pairs - 1)) : -1;
+  const int keys = p.group(min((at.tile + 1) * WQ * 32, pairs) - 1) + 1;
+  const int tiles = (keys + KT - 1) / KT, my_steps = __builtin_amdgcn_readfirstlane(last_query / 32 + (last_query >= 0 ? 1 : 0));
+
+  const int64_t k_row = p.k.row * sizeof(T), v_row = p.v.row * sizeof(T);
+  const char* k_base = HeadOf<T>(p.k, 0, head) + at.first * k_row;
+  const char* v_base = HeadOf<T>(p.v, 0, head) + at.first * v_row;
+  const unsigned lds_at = LdsAddress(lds);
+  // where this lane's chunk of each load lies in a tile; LDS holds the chunks in order, memory gives them turned
+  unsigned off[N];
+  bool none[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int load = wave * N + i;
+    const bool values = load >= STEPS * NC / 2;
+    const int slot = (values ? load - STEPS * NC / 2 : load) * 64 + lane, row = slot / NC;
+    const int c = L::Back(slot % NC, values ? L::WideTurn(row) : L::RowTurn(row));
+    off[i]  = row * (int)(values ? v_row : k_row) + c * 16;
+    none[i] = c >= chunks;
+  }
+  auto request = [&](int tile) {
+    const unsigned to = lds_at + tile % STAGES * STAGE;
+    const int beyond  = at.first + (tile + 1) * KT - p.tokens;  // rows of the tile that are not the tensor's: its last one instead
+    const char *k_tile = k_base + (int64_t)tile * KT * k_row, *v_tile = v_base + (int64_t)tile * KT * v_row;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int load = wave * N + i;
+      const bool values = load >= STEPS * NC / 2;
+      const char* from  = values ? v_tile : k_tile;
+      if (chunks == NC && beyond <= 0) {
+        CopyToLds16(from, off[i], to + load * 1024);
+      } else {
+        const int row  = ((values ? load - STEPS * NC / 2 : load) * 64 + lane) / NC;
+        const int back = max(row - (KT - 1 - beyond), 0) * (int)(values ? v_row : k_row);
+        CopyToLds16(none[i] ? reinterpret_cast<const char*>(kZeros) : from + (int)(off[i] - back), to + load * 1024);
+      }
+    }
+  };
+  auto keys_of = [&](int step) { return lds + step / STEPS % STAGES * STAGE + step % STEPS * L::BYTES; };
+
+  Q rows;
+  rows.Start(HeadOf<T>(p.q, 0, my_head) + (at.first + query) * p.q.row * (int64_t)sizeof(T), chunks, half, p.scale);
+  const Exp<T> ex(p.scale);
+  WaitForAllBut<0>();
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i)
+    if (i < tiles) request(i);
+  if (tiles > 2) {
+    WaitForAllBut<2 * N>();
+  } else if (tiles > 1) {
+    WaitForAllBut<N>();
+  } else {
+    WaitForAllBut<0>();
+  }
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  // before the first step of a tile: it has landed, and everybody is done with the one before the last
+  auto turn = [&](int step) {
+    if (step % STEPS != 0 || step >= tiles * STEPS) return;
+    const int tile = step / STEPS;
+    if (tile + 1 < tiles) {
+      WaitForAllBut<N>();
+    } else {
+      WaitForAllBut<0>();
+    }
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (tile + STAGES - 2 < tiles) request(tile + STAGES - 2);
+  };
+  f32x16 s  = rows.Scores(keys_of(0), lane);
+  float top = Q::Top(s);
+  int step  = 0;
+  // keys that all of the wavefront's queries attend to
+  const int plain_steps = __builtin_amdgcn_readfirstlane(last_query >= 0 ? (first_query + 1) / 32 : 0);
+#pragma unroll 1
+  for (; step < plain_steps; ++step) {
+    rows.Grow(top, ex);
+    turn(step + 1);
+    rows.Soften(s, ex);
+    const f32x16 next = rows.Scores(keys_of(step + 1), lane);
+    rows.Add(s, keys_of(step) + STEPS * L::BYTES, lane);
+    s   = next;
+    top = Q::Top(s);
+  }
+#pragma unroll 1
+  for (; step < tiles * STEPS; ++step) {
+    const unsigned word = Below(query + 1 - step * 32);
+    if (step < my_steps) {
+      Q::Mask(s, word, lane);
+      rows.Grow(Q::Top(s), ex);
+    }
+    turn(step + 1);
+    if (step < my_steps) {
+      rows.Soften(s, ex);
+      const f32x16 next  = rows.Scores(keys_of(step + 1), lane);
+      const char* values = keys_of(step) + STEPS * L::BYTES;
+      if (Q::Unbounded(values, chunks, lane)) {
+        rows.AddChosen(s, word, values, lane);
+      } else {
+        rows.Add(s, values, lane);
+      }
+      s = next;
+    }
+  }
+  const float sum = rows.l + __shfl_xor(rows.l, 32);
+  if (pair0 + (lane & 31) >= pairs) return;
+  char* out = const_cast<char*>(HeadOf<T>(p.o, 0, my_head)) + (at.first + query) * p.o.row * (int64_t)sizeof(T);
+  rows.Store(out, p.d, 1.0f / sum, half);
+}
+
 template <typename T, int D, int WQ, int KG>
 void LaunchBlocks(PackedParams p, hipStream_t stream) {
   p.tiles = (int)((int64_t)p.tokens * p.group.value / (32 * WQ)) + p.sequences + 1;
   hipLaunchKernelGGL((packed_attention_kernel<T, D, WQ, KG>), dim3((unsigned)p.tiles * p.kv_heads), dim3(64 * WQ * KG), 0, stream, p);
 }
 
+template <typename T, int D, int WQ, int STEPS>
+void LaunchRing(PackedParams p, hipStream_t stream) {
+  p.tiles = (int)((int64_t)p.tokens * p.group.value / (32 * WQ)) + p.sequences + 1;
+  hipLaunchKernelGGL((packed_attention_ring_kernel<T, D, WQ, STEPS>), dim3((unsigned)p.tiles * p.kv_heads), dim3(64 * WQ), 0, stream, p);
+}
+
 template <typename T, int D>
 void LaunchTiles(const PackedParams& p, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    static const char* pick = getenv("PICK");
+    const int which = pick ? atoi(pick) : 0;
+    if (which == 0) return LaunchRing<T, D, 8, 2>(p, stream);
+    if (which == 1) return LaunchRing<T, D, 4, 1>(p, stream);
+  }
   // blocks of few pairs where there are few
   const int64_t pairs = (int64_t)p.tokens * p.group.value * p.kv_heads;
   if (pairs >= 256 * 128) {
