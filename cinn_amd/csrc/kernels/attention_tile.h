@@ -119,12 +119,37 @@ struct Dense : Shape<T, D> {
     if (F32) return NC > 8 ? 8 * ((row >> 2) & 1) : 0;
     return NC == 16 ? 4 * (row & 3) : NC == 8 ? 4 * ((row >> 1) & 1) : 0;
   }
-  static __device__ __forceinline__ int KAt(int row, int c) { return (row * NC + Turn(c, RowTurn(row))) * 16; }
+  static __device__ __forceinline__ int KTurn(int row) {
+    return NC % 16 == 0 ? row & 15 : NC % 8 == 0 ? (row >> 1) & 7 : (row >> 2) & 3;
+  }
+  static __device__ __forceinline__ int At(int row, int c) { return (row * NC + Turn(c, RowTurn(row))) * 16; }
+  static __device__ __forceinline__ int KAt(int row, int c) { return (row * NC + Turn(c, KTurn(row))) * 16; }
   static __device__ __forceinline__ int VAt(int row, int c) { return (row * NC + Turn(c, WideTurn(row))) * 16; }
 };
 
 // the bits of a word of 32 keys below `count`
 __device__ __forceinline__ unsigned Below(int count) { return count >= 32 ? ~0u : count <= 0 ? 0u : (1u << count) - 1; }
+
+// registers that hold a lane's sixteen probabilities
+template <typename T>
+struct Held {
+  static constexpr int COUNT = 2;
+  typedef T type __attribute__((ext_vector_type(8)));
+  typedef T pair __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ float AddTwo(T a, T b, float c) {
+    const pair two = {a, b}, ones = {(T)1.0f, (T)1.0f};
+    if constexpr (__is_same(T, _Float16)) {
+      return __builtin_amdgcn_fdot2(two, ones, c, false);
+    } else {
+      return __builtin_amdgcn_fdot2_f32_bf16(two, ones, c, false);
+    }
+  }
+};
+template <>
+struct Held<float> {
+  static constexpr int COUNT = 1;
+  typedef f32x16 type;
+};
 
 // 32 queries of a wavefront, a lane of either half holding one: S^T = K Q^T leaves the lane 16 scores of its query, register
 // r of key 8 (r / 4) + 4 half + r % 4, and O^T = V^T P^T sixteen sums of each 32 elements of d in the same order.
@@ -188,18 +213,39 @@ struct Queries {
       m = top;
     }
   }
-  __device__ __forceinline__ void Soften(f32x16& s, const Exp<T>& ex) {
-    const float base = ex.Base(m);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = ex(s[r], base);
-      l += s[r];
+  // The probabilities of 32 keys as the matrix cores take them: 16-bit ones are rounded, which costs half a step of the type
+  // as the result's own rounding does and is, in numerator and sum alike, all but weighed out; fp32 operands split in two
+  // would take twice the MFMAs.  Two are summed by one dot product with ones.
+  struct Probabilities {
+    typename Held<T>::type g[Held<T>::COUNT];
+    __device__ __forceinline__ float At(int r) const {  // of register r, which is known after unrolling
+      if constexpr (L::F32) {
+        return g[0][r];
+      } else {
+        return (float)g[r / 8][r % 8];
+      }
     }
+  };
+  __device__ __forceinline__ Probabilities Soften(f32x16 s, const Exp<T>& ex) {
+    const float base = ex.Base(m);
+    Probabilities p;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = ex(s[r], base);
+    if constexpr (L::F32) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) l += s[r];
+      p.g[0] = s;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p.g[r / 8][r % 8] = (T)s[r];
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) l = Held<T>::AddTwo(p.g[r / 8][r % 8], p.g[r / 8][r % 8 + 1], l);
+    }
+    return p;
   }
 
-  // sums of 32 keys' values; 16-bit probabilities are rounded on their way into the matrix cores: half a step of the type,
-  // which the result's own rounding has too, at twice (fp16, bf16) the rate that fp32 operands split in two would have
-  __device__ __forceinline__ void Add(const f32x16& s, const char* tile, int lane) {
+  // sums of 32 keys' values
+  __device__ __forceinline__ void Add(const Probabilities& p, const char* tile, int lane) {
     const int half = lane >> 5;
     if constexpr (L::F32) {
 #pragma unroll
@@ -208,15 +254,11 @@ struct Queries {
         for (int r = 0; r < 16; ++r) {
           const int key = 8 * (r >> 2) + 4 * half + (r & 3);
           const float v = *reinterpret_cast<const float*>(tile + L::VAt(key, t * 8 + (lane & 31) / 4) + (lane & 3) * 4);
-          o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[r], o[t], 0, 0, 0);
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p.g[0][r], o[t], 0, 0, 0);
         }
     } else {
-      typedef T vec8 __attribute__((ext_vector_type(8)));
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        vec8 pr;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) pr[e] = (T)s[8 * g + e];
 #pragma unroll
         for (int t = 0; t < L::DT; ++t) {
           // four keys x sixteen d per group of 16 lanes, transposed on the way
@@ -228,7 +270,7 @@ struct Queries {
             part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)at);
           }
           o[t] = Mma<T>::mma(__builtin_bit_cast(u32x4, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7)),
-                             __builtin_bit_cast(u32x4, pr), o[t]);
+                             __builtin_bit_cast(u32x4, p.g[g]), o[t]);
         }
       }
     }
@@ -238,8 +280,11 @@ struct Queries {
   static __device__ __forceinline__ bool Unbounded(const char* tile, int chunks, int lane) {
     constexpr unsigned kExponent = L::F32 ? 0x7f800000u : sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
     bool found = false;
-    for (int at = lane; at < 32 * chunks; at += 64) {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(tile + L::VAt(at / chunks, at % chunks));
+#pragma unroll
+    for (int i = 0; i < L::NC / 2; ++i) {
+      const int at = i * 64 + lane;
+      if (at % L::NC >= chunks) continue;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(tile + L::VAt(at / L::NC, at % L::NC));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         found |= (v[e] & kExponent) == kExponent;
@@ -251,15 +296,17 @@ struct Queries {
 
   // Add for values among which are infinities or NaN, where a probability of zero by the mask must not make 0 * inf: key
   // by key, only where the query attends to it
-  __device__ __forceinline__ void AddChosen(const f32x16& s, unsigned word, const char* tile, int lane) {
+  __device__ __forceinline__ void AddChosen(const Probabilities& p, unsigned word, const char* tile, int lane) {
     const int half = lane >> 5;
+    f32x16 all;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) all[r] = p.At(r);
 #pragma unroll 1
     for (int at = 0; at < 32; ++at) {
       const int owner = at >> 4, reg = at & 15, key = 8 * (reg >> 2) + 4 * owner + (reg & 3);
-      float mine = s[0];
+      float mine = all[0];
 #pragma unroll
-      for (int r = 1; r < 16; ++r) mine = reg == r ? s[r] : mine;
-      mine = (float)(T)mine;
+      for (int r = 1; r < 16; ++r) mine = reg == r ? all[r] : mine;
       const float other = __shfl_xor(mine, 32), prob = half == owner ? mine : other;
       const bool chosen = (word >> key) & 1;
 #pragma unroll
@@ -280,11 +327,11 @@ struct Queries {
     const bool masked = __ballot(word != ~0u) != 0;
     if (masked) Mask(s, word, lane);
     Grow(Top(s), ex);
-    Soften(s, ex);
+    const Probabilities p = Soften(s, ex);
     if (masked && Unbounded(v_tile, chunks, lane)) {
-      AddChosen(s, word, v_tile, lane);
+      AddChosen(p, word, v_tile, lane);
     } else {
-      Add(s, v_tile, lane);
+      Add(p, v_tile, lane);
     }
   }
 

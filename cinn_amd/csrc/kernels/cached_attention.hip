@@ -310,7 +310,7 @@ struct FewPairs {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int key = 16 * (e >> 2) + 4 * (lane >> 4) + (e & 3);
-          const float v = *reinterpret_cast<const float*>(tile + L::KAt(key, 4 * t + ((lane & 15) >> 2)) + (lane & 3) * 4);
+          const float v = *reinterpret_cast<const float*>(tile + L::At(key, 4 * t + ((lane & 15) >> 2)) + (lane & 3) * 4);
 #pragma unroll
           for (int n = 0; n < PT; ++n) o[n][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[n][e >> 2][e & 3], o[n][t], 0, 0, 0);
         }
@@ -326,7 +326,7 @@ struct FewPairs {
         s16x4 part[2];  // four keys x sixteen d per group of 16 lanes, transposed on the way
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const char* at = tile + L::KAt(16 * h + 4 * (lane >> 4) + ((lane & 15) >> 2), 2 * t + ((lane & 3) >> 1)) + (lane & 1) * 8;
+          const char* at = tile + L::At(16 * h + 4 * (lane >> 4) + ((lane & 15) >> 2), 2 * t + ((lane & 3) >> 1)) + (lane & 1) * 8;
           part[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)at);
         }
         const u32x4 v = __builtin_bit_cast(u32x4, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
@@ -366,7 +366,7 @@ struct FewPairs {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int byte = (16 * t + 4 * (lane >> 4) + r) * (int)sizeof(T);
-            const float v  = (float)*reinterpret_cast<const T*>(tile + L::KAt(key, byte >> 4) + (byte & 15));
+            const float v  = (float)*reinterpret_cast<const T*>(tile + L::At(key, byte >> 4) + (byte & 15));
             o[n][t][r]     = chosen ? __builtin_fmaf(prob, v, o[n][t][r]) : o[n][t][r];
           }
       }
@@ -408,10 +408,13 @@ cached_attention_few_kernel(CachedParams p) {
   // rows of whole loads in one page: a load has one base
   const bool even_rows = L::POW2 && chunks == NC && p.page_rows.value % (L::POW2 ? RPL : 1) == 0;
   const int row_bytes  = (int)(p.row * sizeof(T));
-  constexpr int TURNS  = NC == 32 ? 4 : NC == 16 ? 2 : 1;  // places of a row's chunks repeat with every TURNS loads
-  int lane_off[TURNS];
+  constexpr int TURNS  = NC == 32 ? 8 : NC == 16 ? 4 : NC == 8 ? 2 : 1;  // places of a row's chunks repeat with every TURNS loads
+  int k_off[TURNS], v_off[TURNS];
 #pragma unroll
-  for (int j = 0; j < TURNS; ++j) lane_off[j] = lane / NC * row_bytes + L::Back(lane % NC, L::RowTurn(j * RPL + lane / NC)) * 16;
+  for (int j = 0; j < TURNS; ++j) {
+    k_off[j] = lane / NC * row_bytes + L::Back(lane % NC, L::KTurn(j * RPL + lane / NC)) * 16;
+    v_off[j] = lane / NC * row_bytes + L::Back(lane % NC, L::RowTurn(j * RPL + lane / NC)) * 16;
+  }
 
   int64_t at, end;  // this block's items
   Place place;
@@ -479,13 +482,13 @@ cached_attention_few_kernel(CachedParams p) {
         for (int j = 0; j < N; ++j) {
           const unsigned low = __builtin_amdgcn_readlane((unsigned)offset, j * RPL % 32);
           const unsigned high = __builtin_amdgcn_readlane((unsigned)(offset >> 32), j * RPL % 32);
-          CopyToLds16(pages + (int64_t)((uint64_t)high << 32 | low), (unsigned)lane_off[j % TURNS], to + j * 1024);
+          CopyToLds16(pages + (int64_t)((uint64_t)high << 32 | low), (unsigned)(values ? v_off : k_off)[j % TURNS], to + j * 1024);
         }
       } else {
         const Two* rows = reinterpret_cast<const Two*>(mine + ROWS_AT) + stage * 32;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          const int slot = j * 64 + lane, row = slot / NC, c = L::Back(slot % NC, L::RowTurn(row));
+          const int slot = j * 64 + lane, row = slot / NC, c = L::Back(slot % NC, values ? L::RowTurn(row) : L::KTurn(row));
           const char* from = values ? rows[row].v : rows[row].k;
           CopyToLds16(c < chunks ? from + c * 16 : reinterpret_cast<const char*>(kZeros), to + j * 1024);
         }

@@ -168,19 +168,20 @@ packed_attention_kernel(PackedParams p) {
   rows.Store(out, p.d, 1.0f / sum, half);
 }
 
-// 16-bit types: WQ wavefronts of 32 pairs, tiles of 32 STEPS keys in a ring of four in LDS that loads fill directly, one
-// barrier per tile.  A wavefront multiplies the next 32 keys by its queries while it takes the exponentials of the last
+// 16-bit types: WQ x 32 pairs, KG wavefronts for each 32 that take the steps of 32 keys in turn, tiles of 32 STEPS keys in a
+// ring of four in LDS that loads fill directly, one barrier per tile.  A wavefront multiplies the next 32 keys by its queries while it takes the exponentials of the last
 // scores: the matrix cores and the vector unit work side by side, within a wavefront and, two of them to a SIMD, across.
 // Rows behind the last key are rows of the tensor all the same; nothing attends to them.
-template <typename T, int D, int WQ, int STEPS>
-__global__ void __launch_bounds__(64 * WQ, 2)
+template <typename T, int D, int WQ, int KG, int STEPS>
+__global__ void __launch_bounds__(64 * WQ * KG, 2)
 packed_attention_ring_kernel(PackedParams p) {
   typedef Dense<T, D> L;
   typedef Queries<T, D, L> Q;
-  constexpr int KT = 32 * STEPS, NC = L::NC, STAGE = 2 * STEPS * L::BYTES, STAGES = 4;
-  constexpr int N  = STEPS * NC / WQ;  // loads of a wavefront for a tile, whose values lie behind its keys
-  static_assert(N * WQ == STEPS * NC && STAGES * STAGE <= 160 * 1024 && 2 * N < 64);
-  __shared__ __attribute__((aligned(256))) char lds[STAGES * STAGE];
+  constexpr int KT = 32 * STEPS, NC = L::NC, STAGE = 2 * STEPS * L::BYTES, STAGES = 4, CHUNKS = STEPS / 2;
+  constexpr int N  = STEPS * NC / (WQ * KG);  // loads of a wavefront for a tile, whose values lie behind its keys
+  constexpr int MEET = (KG - 1) * WQ * 64 * Q::kRegisters * 4;
+  static_assert(N * WQ * KG == STEPS * NC && CHUNKS % KG == 0 && 2 * N < 64);
+  __shared__ __attribute__((aligned(256))) char lds[STAGES * STAGE > MEET ? STAGES * STAGE : MEET];
 
   const int head = blockIdx.x % p.kv_heads;
   const Found at = Find(p, blockIdx.x / p.kv_heads, 32 * WQ);
@@ -189,14 +190,14 @@ packed_attention_ring_kernel(PackedParams p) {
     return;
   }
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave / WQ, wq = wave % WQ;
   const int chunks = p.d * (int)sizeof(T) / 16, pairs = at.count * p.group.value;
-  const int pair0 = (at.tile * WQ + wave) * 32;
+  const int pair0 = (at.tile * WQ + wq) * 32;
   const int pair = min(pair0 + (lane & 31), pairs - 1);
   const int query = p.group(pair), my_head = head * p.group.value + pair - query * p.group.value;
   const int first_query = p.group(min(pair0, pairs - 1)), last_query = pair0 < pairs ? p.group(min(pair0 + 31, pairs - 1)) : -1;
   const int keys = p.group(min((at.tile + 1) * WQ * 32, pairs) - 1) + 1;
-  const int tiles = (keys + KT - 1) / KT, my_steps = __builtin_amdgcn_readfirstlane(last_query / 32 + (last_query >= 0 ? 1 : 0));
+  const int tiles = (keys + KT - 1) / KT, my_chunks = __builtin_amdgcn_readfirstlane(last_query >= 0 ? last_query / 64 + 1 : 0);
 
   const int64_t k_row = p.k.row * sizeof(T), v_row = p.v.row * sizeof(T);
   const char* k_base = HeadOf<T>(p.k, 0, head) + at.first * k_row;
@@ -210,7 +211,7 @@ packed_attention_ring_kernel(PackedParams p) {
     const int load = wave * N + i;
     const bool values = load >= STEPS * NC / 2;
     const int slot = (values ? load - STEPS * NC / 2 : load) * 64 + lane, row = slot / NC;
-    const int c = L::Back(slot % NC, values ? L::WideTurn(row) : L::RowTurn(row));
+    const int c = L::Back(slot % NC, values ? L::WideTurn(row) : L::KTurn(row));
     off[i]  = row * (int)(values ? v_row : k_row) + c * 16;
     none[i] = c >= chunks;
   }
@@ -234,26 +235,19 @@ packed_attention_ring_kernel(PackedParams p) {
   };
   auto keys_of = [&](int step) { return lds + step / STEPS % STAGES * STAGE + step % STEPS * L::BYTES; };
 
-  Q rows;
-  rows.Start(HeadOf<T>(p.q, 0, my_head) + (at.first + query) * p.q.row * (int64_t)sizeof(T), chunks, half, p.scale);
-  const Exp<T> ex(p.scale);
-  WaitForAllBut<0>();
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i)
     if (i < tiles) request(i);
-  if (tiles > 2) {
-    WaitForAllBut<2 * N>();
-  } else if (tiles > 1) {
-    WaitForAllBut<N>();
-  } else {
-    WaitForAllBut<0>();
-  }
+  Q rows;
+  rows.Start(HeadOf<T>(p.q, 0, my_head) + (at.first + query) * p.q.row * (int64_t)sizeof(T), chunks, half, p.scale);
+  const Exp<T> ex(p.scale);
+  WaitForAllBut<0>();  // the queries are the last that was asked for
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  // before the first step of a tile: it has landed, and everybody is done with the one before the last
-  auto turn = [&](int step) {
-    if (step % STEPS != 0 || step >= tiles * STEPS) return;
-    const int tile = step / STEPS;
+  // before the first chunk of a tile: it has landed, and everybody is done with the one before the last
+  auto turn = [&](int chunk) {
+    if (chunk % CHUNKS != 0 || chunk >= tiles * CHUNKS) return;
+    const int tile = chunk / CHUNKS;
     if (tile + 1 < tiles) {
       WaitForAllBut<N>();
     } else {
@@ -263,40 +257,54 @@ packed_attention_ring_kernel(PackedParams p) {
     asm volatile("" ::: "memory");
     if (tile + STAGES - 2 < tiles) request(tile + STAGES - 2);
   };
-  f32x16 s  = rows.Scores(keys_of(0), lane);
-  float top = Q::Top(s);
-  int step  = 0;
-  // keys that all of the wavefront's queries attend to
-  const int plain_steps = __builtin_amdgcn_readfirstlane(last_query >= 0 ? (first_query + 1) / 32 : 0);
+  f32x16 s[2];
+  s[0] = rows.Scores(keys_of(2 * kg), lane), s[1] = rows.Scores(keys_of(2 * kg + 1), lane);
+  float top = fmaxf(Q::Top(s[0]), Q::Top(s[1]));
+  int chunk = kg;
+  // chunks of keys that all of the wavefront's queries attend to
+  const int plain_chunks = __builtin_amdgcn_readfirstlane(last_query >= 0 ? (first_query + 1) / 64 : 0);
 #pragma unroll 1
-  for (; step < plain_steps; ++step) {
+  for (; chunk < plain_chunks; chunk += KG) {
     rows.Grow(top, ex);
-    turn(step + 1);
-    rows.Soften(s, ex);
-    const f32x16 next = rows.Scores(keys_of(step + 1), lane);
-    rows.Add(s, keys_of(step) + STEPS * L::BYTES, lane);
-    s   = next;
-    top = Q::Top(s);
+    turn(chunk - kg + KG);
+    const typename Q::Probabilities first = rows.Soften(s[0], ex), second = rows.Soften(s[1], ex);
+    const f32x16 next[2] = {rows.Scores(keys_of(2 * (chunk + KG)), lane), rows.Scores(keys_of(2 * (chunk + KG) + 1), lane)};
+    rows.Add(first, keys_of(2 * chunk) + STEPS * L::BYTES, lane);
+    rows.Add(second, keys_of(2 * chunk + 1) + STEPS * L::BYTES, lane);
+    s[0] = next[0], s[1] = next[1];
+    top  = fmaxf(Q::Top(s[0]), Q::Top(s[1]));
   }
 #pragma unroll 1
-  for (; step < tiles * STEPS; ++step) {
-    const unsigned word = Below(query + 1 - step * 32);
-    if (step < my_steps) {
-      Q::Mask(s, word, lane);
-      rows.Grow(Q::Top(s), ex);
+  for (; chunk < tiles * CHUNKS; chunk += KG) {
+    const unsigned word[2] = {Below(query + 1 - chunk * 64), Below(query + 1 - chunk * 64 - 32)};
+    if (chunk < my_chunks) {
+      Q::Mask(s[0], word[0], lane);
+      Q::Mask(s[1], word[1], lane);
+      rows.Grow(fmaxf(Q::Top(s[0]), Q::Top(s[1])), ex);
     }
-    turn(step + 1);
-    if (step < my_steps) {
-      rows.Soften(s, ex);
-      const f32x16 next  = rows.Scores(keys_of(step + 1), lane);
-      const char* values = keys_of(step) + STEPS * L::BYTES;
-      if (Q::Unbounded(values, chunks, lane)) {
-        rows.AddChosen(s, word, values, lane);
-      } else {
-        rows.Add(s, values, lane);
+    turn(chunk - kg + KG);
+    if (chunk < my_chunks) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const typename Q::Probabilities mine = rows.Soften(s[h], ex);
+        const char* values = keys_of(2 * chunk + h) + STEPS * L::BYTES;
+        if (Q::Unbounded(values, chunks, lane)) {
+          rows.AddChosen(mine, word[h], values, lane);
+        } else {
+          rows.Add(mine, values, lane);
+        }
+        s[h] = rows.Scores(keys_of(2 * (chunk + KG) + h), lane);
       }
-      s = next;
     }
+  }
+  if constexpr (KG > 1) {
+    __syncthreads();
+    float* meet = reinterpret_cast<float*>(lds);
+    if (kg > 0) rows.Hand(meet + ((kg - 1) * WQ + wq) * Q::kRegisters * 64, lane);
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll
+    for (int g = 1; g < KG; ++g) rows.Join(meet + ((g - 1) * WQ + wq) * Q::kRegisters * 64, ex, lane);
   }
   const float sum = rows.l + __shfl_xor(rows.l, 32);
   if (pair0 + (lane & 31) >= pairs) return;
@@ -310,10 +318,10 @@ void LaunchBlocks(PackedParams p, hipStream_t stream) {
   hipLaunchKernelGGL((packed_attention_kernel<T, D, WQ, KG>), dim3((unsigned)p.tiles * p.kv_heads), dim3(64 * WQ * KG), 0, stream, p);
 }
 
-template <typename T, int D, int WQ, int STEPS>
+template <typename T, int D, int WQ, int KG, int STEPS>
 void LaunchRing(PackedParams p, hipStream_t stream) {
   p.tiles = (int)((int64_t)p.tokens * p.group.value / (32 * WQ)) + p.sequences + 1;
-  hipLaunchKernelGGL((packed_attention_ring_kernel<T, D, WQ, STEPS>), dim3((unsigned)p.tiles * p.kv_heads), dim3(64 * WQ), 0, stream, p);
+  hipLaunchKernelGGL((packed_attention_ring_kernel<T, D, WQ, KG, STEPS>), dim3((unsigned)p.tiles * p.kv_heads), dim3(64 * WQ * KG), 0, stream, p);
 }
 
 template <typename T, int D>
@@ -321,8 +329,9 @@ void LaunchTiles(const PackedParams& p, hipStream_t stream) {
   if constexpr (sizeof(T) == 2) {
     static const char* pick = getenv("PICK");
     const int which = pick ? atoi(pick) : 0;
-    if (which == 0) return LaunchRing<T, D, 8, 2>(p, stream);
-    if (which == 1) return LaunchRing<T, D, 4, 1>(p, stream);
+    if (which == 0) return LaunchRing<T, D, 8, 1, 2>(p, stream);
+    if (which == 1) return LaunchRing<T, D, 4, 1, 2>(p, stream);
+    if constexpr (D <= 64) { if (which == 2) return LaunchRing<T, D, 4, 2, 4>(p, stream); if (which == 3) return LaunchRing<T, D, 2, 2, 4>(p, stream); }
   }
   // blocks of few pairs where there are few
   const int64_t pairs = (int64_t)p.tokens * p.group.value * p.kv_heads;
