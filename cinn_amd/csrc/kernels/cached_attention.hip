@@ -643,6 +643,196 @@ cached_attention_few_kernel(CachedParams p) {
   }
 }
 
+// More pairs, 16-bit types: WQ x 32 pairs, KG wavefronts for each 32 that take the steps of 32 keys in turn, tiles of 64 keys in
+// a ring of four in LDS that loads fill directly, one barrier per tile; the next scores' MFMAs run beside the exponentials.
+// Page numbers come two tiles ahead of the rows; every wavefront places all 64 rows, a lane each, and requests its share.
+template <typename T, int D, int WQ, int KG>
+__global__ void __launch_bounds__(64 * WQ * KG, 2)
+cached_attention_ring_kernel(CachedParams p) {
+  typedef Dense<T, D> L;
+  typedef Queries<T, D, L> Q;
+  constexpr int STEPS = 2, KT = 32 * STEPS, NC = L::NC, STAGE = 2 * STEPS * L::BYTES, STAGES = 4, WAVES = WQ * KG;
+  constexpr int LOADS = STEPS * NC, N = (LOADS + WAVES - 1) / WAVES;  // for a tile, and a wavefront's; the last is asked for again
+  constexpr int RPL   = L::POW2 ? 64 / NC : 1;                        // rows per load, where that is a whole number
+  constexpr int IDS_AT = STAGES * STAGE, HOLDS_AT = IDS_AT + 8 * 256, ROWS_AT = HOLDS_AT + 64, ALL = ROWS_AT + WAVES * KT * 16;
+  constexpr int MEET   = (KG - 1) * WQ * 64 * Q::kRegisters * 4;
+  static_assert(2 * (N + 1) < 64 && (KG == 1 || KG == STEPS));
+  __shared__ __attribute__((aligned(256))) char lds[ALL > MEET ? ALL : MEET];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave / WQ, wq = wave % WQ;
+  const int chunks = p.d * (int)sizeof(T) / 16, pairs = p.tokens * p.group.value;
+  const Exp<T> ex(p.scale);
+  const unsigned lds_at = LdsAddress(lds);
+  const bool even_rows  = L::POW2 && chunks == NC && p.page_rows.value % RPL == 0;  // a load has one base
+  unsigned lane_off[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int load = min(wave * N + i, LOADS - 1), slot = load % (LOADS / 2) * 64 + lane, row = slot / NC;
+    lane_off[i]    = lane / NC * (int)(p.row * sizeof(T)) + L::Back(slot % NC, load >= LOADS / 2 ? L::WideTurn(row) : L::KTurn(row)) * 16;
+  }
+
+  int64_t at, end;  // this block's items
+  Place place;
+  if (p.blocks > 0) {
+    const int64_t total = Find(p, -1, KT).count, blocks = min((int64_t)p.blocks, total);
+    if (blockIdx.x >= blocks) return;
+    at = total * blockIdx.x / blocks, end = total * (blockIdx.x + 1) / blocks;
+    place = Find(p, at, KT);
+  } else {
+    const int b = blockIdx.x / p.units, length = LengthOf(p, b), tiles = (length + p.tokens + KT - 1) / KT;
+    at = (int64_t)(blockIdx.x % p.units) * (tiles + kEmpty), end = at + tiles + kEmpty;
+    place = {b, length, 0, (int64_t)(tiles + kEmpty) * p.units};
+  }
+#pragma unroll 1
+  while (at < end) {
+    if (at >= place.first + place.count) place = Find(p, at, KT);
+    const int b = __builtin_amdgcn_readfirstlane(place.b), length = __builtin_amdgcn_readfirstlane(place.length);
+    const int keys = length + p.tokens, tiles = (keys + KT - 1) / KT;
+    const int64_t inside = at - place.first, items = tiles + kEmpty;
+    const int unit = __builtin_amdgcn_readfirstlane((int)(inside / items)), item0 = __builtin_amdgcn_readfirstlane((int)(inside - unit * items));
+    const int item1 = __builtin_amdgcn_readfirstlane((int)min(items, item0 + end - at));
+    const int tile0 = max(item0 - kEmpty, 0), tile1 = item1 - kEmpty;
+    at += item1 - item0;
+    if (tile0 >= tile1) continue;
+    const int head = unit % p.kv_heads, pair0 = (unit / p.kv_heads * WQ + wq) * 32;
+    const int pair = min(pair0 + (lane & 31), pairs - 1), token = p.group(pair), my_head = head * p.group.value + pair - token * p.group.value;
+    const char* k_new = HeadOf<T>(p.k, b, head);
+    const char* v_new = HeadOf<T>(p.v, b, head);
+    const int* table  = p.table + (int64_t)b * p.columns;
+
+    auto request_pages = [&](int tile) {
+      const int key = min(min(tile, tile1 - 1) * KT + lane, max(length - 1, 0));
+      CopyToLds4(table + p.page_rows(key), lds_at + IDS_AT + tile % 8 * 256);
+    };
+    int clean = tile1;  // the first tile with a row of the cache that is none
+    struct Two { const char *k, *v; };
+    auto request = [&](int tile) {
+      const int key  = tile * KT + lane;
+      const int page = *reinterpret_cast<const int*>(lds + IDS_AT + tile % 8 * 256 + lane * 4);
+      const bool good = key < length && page >= 0 && page < p.pages;
+      const int64_t offset = good ? (page * p.page + (key - p.page_rows(key) * p.page_rows.value) * p.row + head * p.head) * (int64_t)sizeof(T) : 0;
+      const unsigned long long word = __ballot(good || (key >= length && key < keys));
+      // every wavefront finds and writes the same
+      *reinterpret_cast<unsigned long long*>(lds + HOLDS_AT + tile % 8 * 8) = word;
+      if (tile * KT + KT <= length && word != ~0ull) clean = min(clean, tile);
+      const unsigned to = lds_at + tile % STAGES * STAGE;
+      if (even_rows && __ballot(good) == ~0ull) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int load = min(wave * N + i, LOADS - 1), row = load % (LOADS / 2) * RPL;
+          const unsigned low = __builtin_amdgcn_readlane((unsigned)offset, row);
+          const unsigned high = __builtin_amdgcn_readlane((unsigned)(offset >> 32), row);
+          CopyToLds16((load >= LOADS / 2 ? p.v_pages : p.k_pages) + (int64_t)((uint64_t)high << 32 | low), lane_off[i], to + load * 1024);
+        }
+      } else {
+        // the rows' addresses by way of LDS
+        Two row = {reinterpret_cast<const char*>(kZeros), reinterpret_cast<const char*>(kZeros)};
+        if (good) row = {p.k_pages + offset, p.v_pages + offset};
+        if (key >= length && key < keys)
+          row = {k_new + (key - length) * p.k.row * (int64_t)sizeof(T), v_new + (key - length) * p.v.row * (int64_t)sizeof(T)};
+        Two* rows = reinterpret_cast<Two*>(lds + ROWS_AT + wave * KT * 16);
+        rows[lane] = row;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int load = min(wave * N + i, LOADS - 1), slot = load % (LOADS / 2) * 64 + lane, r = slot / NC;
+          const bool values = load >= LOADS / 2;
+          const int c = L::Back(slot % NC, values ? L::WideTurn(r) : L::KTurn(r));
+          const char* from = values ? rows[r].v : rows[r].k;
+          CopyToLds16(c < chunks ? from + c * 16 : reinterpret_cast<const char*>(kZeros), to + load * 1024);
+        }
+      }
+    };
+    auto keys_of = [&](int step) { return lds + step / STEPS % STAGES * STAGE + step % STEPS * L::BYTES; };
+    auto values_of = [&](int step) { return keys_of(step) + STEPS * L::BYTES; };
+
+    request_pages(tile0);
+    request_pages(tile0 + 1);
+    WaitForAllBut<0>();
+#pragma unroll 1
+    for (int i = 0; i < STAGES - 1 && tile0 + i < tile1; ++i) {
+      if (i == 2) WaitForAllBut<N + 1>();  // page numbers that were asked for before the first rows
+      request_pages(tile0 + i + 2);
+      request(tile0 + i);
+    }
+    const unsigned long long seen = SeenBy(p, b, token);
+    Q rows;
+    rows.Start(HeadOf<T>(p.q, b, my_head) + token * p.q.row * (int64_t)sizeof(T), chunks, lane >> 5, p.scale);
+    WaitForAllBut<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    // before the first step of a tile: it has landed, and everybody is done with the one before the last
+    auto turn = [&](int step) {
+      if (step % STEPS != 0 || step >= tile1 * STEPS) return;
+      const int tile = step / STEPS;
+      if (tile + 1 < tile1) {
+        WaitForAllBut<N + 1>();
+      } else {
+        WaitForAllBut<0>();
+      }
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (tile + STAGES - 2 < tile1) {
+        request_pages(tile + STAGES);
+        request(tile + STAGES - 2);
+      }
+    };
+    int step  = tile0 * STEPS + kg;
+    f32x16 s  = rows.Scores(keys_of(step), lane);
+    float top = Q::Top(s);
+    // steps of cached keys only, for pairs that are tokens
+    const int plain_steps = pair0 < pairs && __ballot(seen == 0) == 0 ? length / 32 : 0, steps = tile1 * STEPS;
+    const int my_steps    = pair0 < pairs ? min(steps, (keys + 31) / 32) : 0;
+    auto word_of = [&](int n) {
+      const int j0  = n * 32 - length;
+      unsigned word = j0 >= 0 ? (unsigned)(seen >> min(j0, 63)) : j0 <= -32 ? ~0u : (unsigned)(seen << -j0) | Below(-j0);
+      word &= *reinterpret_cast<const unsigned*>(lds + HOLDS_AT + n / STEPS % 8 * 8 + n % STEPS * 4);
+      return seen == 0 ? 0u : word;
+    };
+    auto open = [&] {  // the step's scores are complete
+      if (step >= min(plain_steps, clean * STEPS)) {
+        Q::Mask(s, word_of(step), lane);
+        top = Q::Top(s);
+      }
+      rows.Grow(top, ex);
+    };
+#pragma unroll 1
+    for (; step < steps; step += KG) {
+      if (step < my_steps) open();
+      turn(step - kg + KG);
+      if (step >= my_steps) continue;
+      if (step >= min(plain_steps, clean * STEPS) && Q::Unbounded(values_of(step), chunks, lane)) break;
+      const typename Q::Probabilities mine = rows.Soften(s, ex);
+      s = rows.Scores(keys_of(step + KG), lane);
+      rows.Add(mine, values_of(step), lane);
+      top = Q::Top(s);
+    }
+    // from the first step on whose values a mask alone does not keep out; it has been opened
+#pragma unroll 1
+    for (bool opened = true; step < steps; step += KG, opened = false) {
+      if (!opened) {
+        if (step < my_steps) open();
+        turn(step - kg + KG);
+      }
+      if (step >= my_steps) continue;
+      rows.AddChosen(rows.Soften(s, ex), word_of(step), values_of(step), lane);
+      s   = rows.Scores(keys_of(step + KG), lane);
+      top = Q::Top(s);
+    }
+    __syncthreads();
+    if constexpr (KG > 1) {
+      float* meet = reinterpret_cast<float*>(lds);
+      if (kg > 0) rows.Hand(meet + ((kg - 1) * WQ + wq) * Q::kRegisters * 64, lane);
+      __syncthreads();
+      if (kg == 0) {
+#pragma unroll
+        for (int g = 1; g < KG; ++g) rows.Join(meet + ((g - 1) * WQ + wq) * Q::kRegisters * 64, ex, lane);
+      }
+      __syncthreads();  // the next unit's tiles may overwrite what was read here
+    }
+    if (kg == 0) Finish<T, D>(p, rows, b, head, pair0, lane, tile0 == 0, tile1 == tiles, WQ, wq, seen);
+  }
+}
+
 // Units whose tiles several blocks had: a wavefront takes four registers of the lanes of TILE pairs, four consecutive elements
 // of d.  RUNS: of TILE pairs in a block's unit.
 template <typename T, int D, int TILE, int RUNS>
@@ -732,6 +922,13 @@ void LaunchFew(CachedParams p, hipStream_t stream) {
   LaunchJoin<T, D, 16, PT>(p, 32 * kWaves, stream);
 }
 
+template <typename T, int D, int WQ, int KG>
+void LaunchRing(CachedParams p, hipStream_t stream) {
+  const int blocks = Divide<D>(p, 32, WQ, 64, stream);
+  hipLaunchKernelGGL((cached_attention_ring_kernel<T, D, WQ, KG>), dim3((unsigned)blocks), dim3(64 * WQ * KG), 0, stream, p);
+  LaunchJoin<T, D, 32, WQ>(p, 64, stream);
+}
+
 template <typename T, int D>
 void LaunchTiles(CachedParams p, hipStream_t stream) {
   const int pairs = p.tokens * p.group.value;
@@ -739,10 +936,18 @@ void LaunchTiles(CachedParams p, hipStream_t stream) {
     LaunchFew<T, D, 1>(p, stream);
   } else if (pairs <= 32) {
     LaunchFew<T, D, 2>(p, stream);
-  } else {
+  } else if constexpr (sizeof(T) == 4) {
     const int blocks = Divide<D>(p, 32, 4, 64, stream);
     hipLaunchKernelGGL((cached_attention_kernel<T, D, 4, 2>), dim3((unsigned)blocks), dim3(512), 0, stream, p);
     LaunchJoin<T, D, 32, 4>(p, 64, stream);
+  } else if (pairs <= 64) {
+    LaunchRing<T, D, 2, 2>(p, stream);
+  } else if (pairs <= 128) {
+    LaunchRing<T, D, 4, 2>(p, stream);
+  } else if ((pairs + 191) / 192 * 6 < (pairs + 255) / 256 * 8) {
+    LaunchRing<T, D, 6, 1>(p, stream);
+  } else {
+    LaunchRing<T, D, 8, 1>(p, stream);
   }
 }
 

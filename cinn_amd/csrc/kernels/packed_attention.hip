@@ -177,10 +177,10 @@ __global__ void __launch_bounds__(64 * WQ * KG, 2)
 packed_attention_ring_kernel(PackedParams p) {
   typedef Dense<T, D> L;
   typedef Queries<T, D, L> Q;
-  constexpr int KT = 32 * STEPS, NC = L::NC, STAGE = 2 * STEPS * L::BYTES, STAGES = 4, CHUNKS = STEPS / 2;
+  constexpr int KT = 32 * STEPS, NC = L::NC, STAGE = 2 * STEPS * L::BYTES, STAGES = 4;
   constexpr int N  = STEPS * NC / (WQ * KG);  // loads of a wavefront for a tile, whose values lie behind its keys
   constexpr int MEET = (KG - 1) * WQ * 64 * Q::kRegisters * 4;
-  static_assert(N * WQ * KG == STEPS * NC && CHUNKS % KG == 0 && 2 * N < 64);
+  static_assert(N * WQ * KG == STEPS * NC && STEPS % KG == 0 && 2 * N < 64);
   __shared__ __attribute__((aligned(256))) char lds[STAGES * STAGE > MEET ? STAGES * STAGE : MEET];
 
   const int head = blockIdx.x % p.kv_heads;
@@ -197,7 +197,7 @@ packed_attention_ring_kernel(PackedParams p) {
   const int query = p.group(pair), my_head = head * p.group.value + pair - query * p.group.value;
   const int first_query = p.group(min(pair0, pairs - 1)), last_query = pair0 < pairs ? p.group(min(pair0 + 31, pairs - 1)) : -1;
   const int keys = p.group(min((at.tile + 1) * WQ * 32, pairs) - 1) + 1;
-  const int tiles = (keys + KT - 1) / KT, my_chunks = __builtin_amdgcn_readfirstlane(last_query >= 0 ? last_query / 64 + 1 : 0);
+  const int tiles = (keys + KT - 1) / KT, my_steps = __builtin_amdgcn_readfirstlane(last_query >= 0 ? last_query / 32 + 1 : 0);
 
   const int64_t k_row = p.k.row * sizeof(T), v_row = p.v.row * sizeof(T);
   const char* k_base = HeadOf<T>(p.k, 0, head) + at.first * k_row;
@@ -244,10 +244,10 @@ packed_attention_ring_kernel(PackedParams p) {
   WaitForAllBut<0>();  // the queries are the last that was asked for
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  // before the first chunk of a tile: it has landed, and everybody is done with the one before the last
-  auto turn = [&](int chunk) {
-    if (chunk % CHUNKS != 0 || chunk >= tiles * CHUNKS) return;
-    const int tile = chunk / CHUNKS;
+  // before the first step of a tile: it has landed, and everybody is done with the one before the last
+  auto turn = [&](int step) {
+    if (step % STEPS != 0 || step >= tiles * STEPS) return;
+    const int tile = step / STEPS;
     if (tile + 1 < tiles) {
       WaitForAllBut<N>();
     } else {
@@ -257,45 +257,41 @@ packed_attention_ring_kernel(PackedParams p) {
     asm volatile("" ::: "memory");
     if (tile + STAGES - 2 < tiles) request(tile + STAGES - 2);
   };
-  f32x16 s[2];
-  s[0] = rows.Scores(keys_of(2 * kg), lane), s[1] = rows.Scores(keys_of(2 * kg + 1), lane);
-  float top = fmaxf(Q::Top(s[0]), Q::Top(s[1]));
-  int chunk = kg;
-  // chunks of keys that all of the wavefront's queries attend to
-  const int plain_chunks = __builtin_amdgcn_readfirstlane(last_query >= 0 ? (first_query + 1) / 64 : 0);
-#pragma unroll 1
-  for (; chunk < plain_chunks; chunk += KG) {
+  f32x16 s  = rows.Scores(keys_of(kg), lane);
+  float top = Q::Top(s);
+  int step  = kg;
+  // steps of keys that all of the wavefront's queries attend to
+  const int plain_steps = __builtin_amdgcn_readfirstlane(last_query >= 0 ? (first_query + 1) / 32 : 0);
+  auto open = [&] {  // the step's scores are complete
+    if (step >= plain_steps) {
+      Q::Mask(s, Below(query + 1 - step * 32), lane);
+      top = Q::Top(s);
+    }
     rows.Grow(top, ex);
-    turn(chunk - kg + KG);
-    const typename Q::Probabilities first = rows.Soften(s[0], ex), second = rows.Soften(s[1], ex);
-    const f32x16 next[2] = {rows.Scores(keys_of(2 * (chunk + KG)), lane), rows.Scores(keys_of(2 * (chunk + KG) + 1), lane)};
-    rows.Add(first, keys_of(2 * chunk) + STEPS * L::BYTES, lane);
-    rows.Add(second, keys_of(2 * chunk + 1) + STEPS * L::BYTES, lane);
-    s[0] = next[0], s[1] = next[1];
-    top  = fmaxf(Q::Top(s[0]), Q::Top(s[1]));
-  }
+  };
+  auto values_of = [&](int n) { return keys_of(n) + STEPS * L::BYTES; };
 #pragma unroll 1
-  for (; chunk < tiles * CHUNKS; chunk += KG) {
-    const unsigned word[2] = {Below(query + 1 - chunk * 64), Below(query + 1 - chunk * 64 - 32)};
-    if (chunk < my_chunks) {
-      Q::Mask(s[0], word[0], lane);
-      Q::Mask(s[1], word[1], lane);
-      rows.Grow(fmaxf(Q::Top(s[0]), Q::Top(s[1])), ex);
+  for (; step < tiles * STEPS; step += KG) {
+    if (step < my_steps) open();
+    turn(step - kg + KG);
+    if (step >= my_steps) continue;
+    if (step >= plain_steps && Q::Unbounded(values_of(step), chunks, lane)) break;
+    const typename Q::Probabilities mine = rows.Soften(s, ex);
+    s = rows.Scores(keys_of(step + KG), lane);
+    rows.Add(mine, values_of(step), lane);
+    top = Q::Top(s);
+  }
+  // from the first step on whose values a mask alone does not keep out; it has been opened
+#pragma unroll 1
+  for (bool opened = true; step < tiles * STEPS; step += KG, opened = false) {
+    if (!opened) {
+      if (step < my_steps) open();
+      turn(step - kg + KG);
     }
-    turn(chunk - kg + KG);
-    if (chunk < my_chunks) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const typename Q::Probabilities mine = rows.Soften(s[h], ex);
-        const char* values = keys_of(2 * chunk + h) + STEPS * L::BYTES;
-        if (Q::Unbounded(values, chunks, lane)) {
-          rows.AddChosen(mine, word[h], values, lane);
-        } else {
-          rows.Add(mine, values, lane);
-        }
-        s[h] = rows.Scores(keys_of(2 * (chunk + KG) + h), lane);
-      }
-    }
+    if (step >= my_steps) continue;
+    rows.AddChosen(rows.Soften(s, ex), Below(query + 1 - step * 32), values_of(step), lane);
+    s   = rows.Scores(keys_of(step + KG), lane);
+    top = Q::Top(s);
   }
   if constexpr (KG > 1) {
     __syncthreads();
@@ -330,8 +326,8 @@ void LaunchTiles(const PackedParams& p, hipStream_t stream) {
     static const char* pick = getenv("PICK");
     const int which = pick ? atoi(pick) : 0;
     if (which == 0) return LaunchRing<T, D, 8, 1, 2>(p, stream);
-    if (which == 1) return LaunchRing<T, D, 4, 1, 2>(p, stream);
-    if constexpr (D <= 64) { if (which == 2) return LaunchRing<T, D, 4, 2, 4>(p, stream); if (which == 3) return LaunchRing<T, D, 2, 2, 4>(p, stream); }
+    if (which == 2) return LaunchRing<T, D, 4, 1, 1>(p, stream);
+    if (which == 3) return LaunchRing<T, D, 4, 2, 2>(p, stream);
   }
   // blocks of few pairs where there are few
   const int64_t pairs = (int64_t)p.tokens * p.group.value * p.kv_heads;
