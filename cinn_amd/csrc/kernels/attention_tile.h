@@ -135,15 +135,6 @@ template <typename T>
 struct Held {
   static constexpr int COUNT = 2;
   typedef T type __attribute__((ext_vector_type(8)));
-  typedef T pair __attribute__((ext_vector_type(2)));
-  static __device__ __forceinline__ float AddTwo(T a, T b, float c) {
-    const pair two = {a, b}, ones = {(T)1.0f, (T)1.0f};
-    if constexpr (__is_same(T, _Float16)) {
-      return __builtin_amdgcn_fdot2(two, ones, c, false);
-    } else {
-      return __builtin_amdgcn_fdot2_f32_bf16(two, ones, c, false);
-    }
-  }
 };
 template <>
 struct Held<float> {
@@ -214,8 +205,8 @@ struct Queries {
     }
   }
   // The probabilities of 32 keys as the matrix cores take them: 16-bit ones are rounded, which costs half a step of the type
-  // as the result's own rounding does and is, in numerator and sum alike, all but weighed out; fp32 operands split in two
-  // would take twice the MFMAs.  Two are summed by one dot product with ones.
+  // as the result's own rounding does; fp32 operands split in two would take twice the MFMAs.  They are summed before (in twos
+  // by dot products with ones: half the instructions, and 3% slower over 16384 keys).
   struct Probabilities {
     typename Held<T>::type g[Held<T>::COUNT];
     __device__ __forceinline__ float At(int r) const {  // of register r, which is known after unrolling
@@ -231,15 +222,13 @@ struct Queries {
     Probabilities p;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = ex(s[r], base);
-    if constexpr (L::F32) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) l += s[r];
+    for (int r = 0; r < 16; ++r) l += s[r];
+    if constexpr (L::F32) {
       p.g[0] = s;
     } else {
 #pragma unroll
       for (int r = 0; r < 16; ++r) p.g[r / 8][r % 8] = (T)s[r];
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) l = Held<T>::AddTwo(p.g[r / 8][r % 8], p.g[r / 8][r % 8 + 1], l);
     }
     return p;
   }
@@ -368,6 +357,179 @@ struct Queries {
         for (int e = 0; e < 4; ++e) four[e] = (T)(o[t][4 * i + e] * factor);
         if (at < d) __builtin_memcpy(row + at * sizeof(T), four, sizeof(four));
       }
+  }
+};
+
+// 16 x PT queries of a wavefront against 32 keys at a time, where there are few: S^T = K Q^T by MFMAs of 16 keys x 16 pairs, a
+// lane holding the scores of pair lane % 16 (+ 16 per pair tile) for the keys 16 h + 4 (lane / 16) + r, which is, as it lies, the
+// second operand of O^T = V^T P^T.
+template <typename T, int D, int PT>
+struct FewPairs {
+  typedef Dense<T, D> L;
+  static constexpr bool F32 = L::F32;
+  static constexpr int STEPS = L::NC / 4, DT = D / 16;
+  u32x4 q[PT][STEPS];
+  float m[PT], l[PT];  // l: of this lane's keys only
+  f32x4 o[PT][DT];     // d = 16 t + 4 (lane / 16) + r
+
+  // the chunk of a row that a lane multiplies in step i: halves of a wavefront take neighbouring ones, whose place in LDS
+  // differs in the lowest bit
+  static __device__ __forceinline__ int ChunkOf(int i, int lane) { return 4 * i + 2 * ((lane >> 4) & 1) + (lane >> 5); }
+
+  __device__ __forceinline__ void Start(int tile, const char* row, int chunks, int lane, float scale) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      q[tile][i] = u32x4{0, 0, 0, 0};
+      if (ChunkOf(i, lane) < chunks) q[tile][i] = Signed<T>(LoadAny<T>(row + ChunkOf(i, lane) * 16), scale);
+    }
+    m[tile] = -__builtin_inff(), l[tile] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[tile][t] = f32x4{0, 0, 0, 0};
+  }
+  static __device__ __forceinline__ f32x4 Multiply(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (F32) {
+      const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+      return c;
+    } else {
+      typedef typename cinn_hip_kernels::flex::Half16<T> H;
+      return H::mfma(__builtin_bit_cast(typename H::vec8, a), __builtin_bit_cast(typename H::vec8, b), c);
+    }
+  }
+  __device__ __forceinline__ void Scores(f32x4 (&s)[PT][2], const char* tile, int lane) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int n = 0; n < PT; ++n) s[n][h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const u32x4 k = *reinterpret_cast<const u32x4*>(tile + L::KAt(16 * h + (lane & 15), ChunkOf(i, lane)));
+#pragma unroll
+        for (int n = 0; n < PT; ++n) s[n][h] = Multiply(k, q[n][i], s[n][h]);
+      }
+    }
+  }
+  static __device__ __forceinline__ void Mask(f32x4 (&s)[2], unsigned word, int lane) {
+    word >>= 4 * (lane >> 4);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (!((word >> (16 * h + r)) & 1)) s[h][r] = -__builtin_inff();
+  }
+  // as Queries::Soften
+  __device__ __forceinline__ void Soften(int tile, f32x4 (&s)[2], const Exp<T>& ex) {
+    float top = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e >> 2][e & 3]);
+    if (__ballot((top - m[tile]) * ex.c > 8.0f)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(m[tile], fmaxf(top, __shfl_xor(top, 32)));
+      const float keep = ex(m[tile], ex.Base(top));
+      l[tile] *= keep;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) o[tile][t] *= keep;
+      m[tile] = top;
+    }
+    const float base = ex.Base(m[tile]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      s[e >> 2][e & 3] = ex(s[e >> 2][e & 3], base);
+      l[tile] += s[e >> 2][e & 3];
+    }
+  }
+  // 16-bit probabilities round on their way into the matrix cores, as in Queries::Add
+  __device__ __forceinline__ void Add(const f32x4 (&s)[PT][2], const char* tile, int lane) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int key = 16 * (e >> 2) + 4 * (lane >> 4) + (e & 3);
+          const float v = *reinterpret_cast<const float*>(tile + L::At(key, 4 * t + ((lane & 15) >> 2)) + (lane & 3) * 4);
+#pragma unroll
+          for (int n = 0; n < PT; ++n) o[n][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[n][e >> 2][e & 3], o[n][t], 0, 0, 0);
+        }
+    } else {
+      typedef T vec8 __attribute__((ext_vector_type(8)));
+      vec8 pr[PT];
+#pragma unroll
+      for (int n = 0; n < PT; ++n)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pr[n][e] = (T)s[n][e >> 2][e & 3];
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        s16x4 part[2];  // four keys x sixteen d per group of 16 lanes, transposed on the way
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const char* at = tile + L::At(16 * h + 4 * (lane >> 4) + ((lane & 15) >> 2), 2 * t + ((lane & 3) >> 1)) + (lane & 1) * 8;
+          part[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)at);
+        }
+        const u32x4 v = __builtin_bit_cast(u32x4, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int n = 0; n < PT; ++n) o[n][t] = Multiply(v, __builtin_bit_cast(u32x4, pr[n]), o[n][t]);
+      }
+    }
+  }
+  // as Queries::Unbounded and Queries::AddChosen
+  static __device__ __forceinline__ bool Unbounded(const char* tile, int lane) {
+    constexpr unsigned kExponent = F32 ? 0x7f800000u : __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < L::NC / 2; ++i) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(tile + (i * 64 + lane) * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        found |= (v[e] & kExponent) == kExponent;
+        if (!F32) found |= (v[e] >> 16 & kExponent) == kExponent;
+      }
+    }
+    return __ballot(found) != 0;
+  }
+  __device__ __forceinline__ void AddChosen(const f32x4 (&s)[PT][2], const unsigned (&word)[PT], const char* tile, int lane) {
+#pragma unroll 1
+    for (int key = 0; key < 32; ++key) {
+      const int reg = (key >> 4) * 4 + (key & 3), owner = (key & 15) >> 2;
+#pragma unroll
+      for (int n = 0; n < PT; ++n) {
+        float prob = s[n][0][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) prob = reg == e ? s[n][e >> 2][e & 3] : prob;
+        prob = __shfl((float)(T)prob, owner * 16 + (lane & 15));
+        const bool chosen = (word[n] >> key) & 1;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int byte = (16 * t + 4 * (lane >> 4) + r) * (int)sizeof(T);
+            const float v  = (float)*reinterpret_cast<const T*>(tile + L::At(key, byte >> 4) + (byte & 15));
+            o[n][t][r]     = chosen ? __builtin_fmaf(prob, v, o[n][t][r]) : o[n][t][r];
+          }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void Store(int tile, char* row, int d, float factor, int lane) const {
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      const int at = 16 * t + 4 * (lane >> 4);
+      T four[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) four[r] = (T)(o[tile][t][r] * factor);
+      if (at < d) __builtin_memcpy(row + at * sizeof(T), four, sizeof(four));
+    }
+  }
+
+  // what another wavefront has of one pair tile, [register][lane]
+  static constexpr int kRegisters = DT * 4 + 2;
+  __device__ __forceinline__ void Hand(int tile, float* to, int lane) const {
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) to[(t * 4 + r) * 64 + lane] = o[tile][t][r];
+    to[(kRegisters - 2) * 64 + lane] = m[tile];
+    to[(kRegisters - 1) * 64 + lane] = l[tile];
   }
 };
 

@@ -11,7 +11,6 @@
 #include <algorithm>
 #include <climits>
 #include <cstdint>
-#include <cstdlib>
 
 #include "cinn_hip_runtime.h"
 #include "kernels/attention_tile.h"
@@ -76,98 +75,6 @@ __device__ void ClearRest(const PackedParams& p, int head, int index, int blocks
   }
 }
 
-// D: d rounded up to an instance; WQ x 32 pairs per block, KG groups of wavefronts that take the tiles' keys in turn
-template <typename T, int D, int WQ, int KG>
-__global__ void __launch_bounds__(64 * WQ * KG, 2)
-packed_attention_kernel(PackedParams p) {
-  typedef Queries<T, D> Q;
-  typedef Padded<T, D> L;
-  constexpr int THREADS = 64 * WQ * KG, KT = 32 * KG, NC = L::NC;
-  constexpr int V_AT = KT * L::K_PITCH, STAGE = V_AT + KT * L::V_PITCH;
-  constexpr int MEET = (KG - 1) * WQ * 64 * Q::kRegisters * 4;
-  __shared__ __attribute__((aligned(256))) char lds[2 * STAGE > MEET ? 2 * STAGE : MEET];
-
-  // consecutive blocks, which are on different XCDs, take different key heads
-  const int head = blockIdx.x % p.kv_heads;
-  const Found at = Find(p, blockIdx.x / p.kv_heads, 32 * WQ);
-  if (at.count == 0) {
-    ClearRest<T>(p, head, at.tile, at.more);
-    return;
-  }
-  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave / WQ, wq = wave % WQ;
-  const int chunks = p.d * (int)sizeof(T) / 16, pairs = at.count * p.group.value;
-  const int pair0 = (at.tile * WQ + wq) * 32;  // of this wavefront
-  const int pair = min(pair0 + (lane & 31), pairs - 1);
-  const int query = p.group(pair), my_head = head * p.group.value + pair - query * p.group.value;
-  const int first_query = p.group(min(pair0, pairs - 1)), last_query = pair0 < pairs ? p.group(min(pair0 + 31, pairs - 1)) : -1;
-  const int keys = p.group(min((at.tile + 1) * WQ * 32, pairs) - 1) + 1;
-
-  const int64_t k_row = p.k.row * sizeof(T), v_row = p.v.row * sizeof(T);
-  const char* k_base = HeadOf<T>(p.k, 0, head) + at.first * k_row;
-  const char* v_base = HeadOf<T>(p.v, 0, head) + at.first * v_row;
-  constexpr int N = (KT * NC + THREADS - 1) / THREADS;
-  u32x4 kr[N], vr[N];
-  auto load = [&](int key0) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (tid + i * THREADS) % NC, row = (tid + i * THREADS) / NC, key = key0 + row;
-      kr[i] = vr[i] = u32x4{0, 0, 0, 0};
-      if (key < keys && c < chunks && row < KT) {
-        kr[i] = LoadAny<T>(k_base + key * k_row + c * 16);
-        vr[i] = LoadAny<T>(v_base + key * v_row + c * 16);
-      }
-    }
-  };
-  auto store = [&](char* stage) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (tid + i * THREADS) % NC, row = (tid + i * THREADS) / NC;
-      if (KT * NC % THREADS == 0 || row < KT) {
-        *reinterpret_cast<u32x4*>(stage + row * L::K_PITCH + c * 16)        = kr[i];
-        *reinterpret_cast<u32x4*>(stage + V_AT + row * L::V_PITCH + c * 16) = vr[i];
-      }
-    }
-  };
-
-  load(0);
-  Q rows;
-  rows.Start(HeadOf<T>(p.q, 0, my_head) + (at.first + query) * p.q.row * (int64_t)sizeof(T), chunks, half, p.scale);
-  const Exp<T> ex(p.scale);
-  store(lds);
-  __syncthreads();
-  const int tiles = (keys + KT - 1) / KT;
-#pragma unroll 1
-  for (int kt = 0; kt < tiles; ++kt) {
-    const char* cur = lds + (kt & 1) * STAGE;
-    if (kt + 1 < tiles) load((kt + 1) * KT);
-    const int key0 = kt * KT + kg * 32;
-    if (key0 <= last_query) {
-      const unsigned word = key0 + 31 <= first_query ? ~0u : Below(query + 1 - key0);
-      rows.Step(cur + kg * 32 * L::K_PITCH, cur + V_AT + kg * 32 * L::V_PITCH, word, chunks, ex, lane);
-    }
-    if (kt + 1 < tiles) {
-      store(lds + ((kt + 1) & 1) * STAGE);
-      __syncthreads();
-    }
-  }
-
-  if constexpr (KG > 1) {
-    __syncthreads();
-    float* meet = reinterpret_cast<float*>(lds);
-    if (kg > 0) rows.Hand(meet + ((kg - 1) * WQ + wq) * Q::kRegisters * 64, lane);
-    __syncthreads();
-    if (kg > 0) return;
-#pragma unroll
-    for (int g = 1; g < KG; ++g) rows.Join(meet + ((g - 1) * WQ + wq) * Q::kRegisters * 64, ex, lane);
-  }
-  // both halves of the wavefront hold this pair
-  const float sum = rows.l + __shfl_xor(rows.l, 32);
-  if (pair0 + (lane & 31) >= pairs) return;
-  char* out = const_cast<char*>(HeadOf<T>(p.o, 0, my_head)) + (at.first + query) * p.o.row * (int64_t)sizeof(T);
-  rows.Store(out, p.d, 1.0f / sum, half);
-}
-
 // 16-bit types: WQ x 32 pairs, KG wavefronts for each 32 that take the steps of 32 keys in turn, tiles of 32 STEPS keys in a
 // ring of four in LDS that loads fill directly, one barrier per tile.  A wavefront multiplies the next 32 keys by its queries while it takes the exponentials of the last
 // scores: the matrix cores and the vector unit work side by side, within a wavefront and, two of them to a SIMD, across.
@@ -178,9 +85,9 @@ packed_attention_ring_kernel(PackedParams p) {
   typedef Dense<T, D> L;
   typedef Queries<T, D, L> Q;
   constexpr int KT = 32 * STEPS, NC = L::NC, STAGE = 2 * STEPS * L::BYTES, STAGES = 4;
-  constexpr int N  = STEPS * NC / (WQ * KG);  // loads of a wavefront for a tile, whose values lie behind its keys
+  constexpr int LOADS = STEPS * NC, N = (LOADS + WQ * KG - 1) / (WQ * KG);  // for a tile, its values behind its keys, and a wavefront's
   constexpr int MEET = (KG - 1) * WQ * 64 * Q::kRegisters * 4;
-  static_assert(N * WQ * KG == STEPS * NC && STEPS % KG == 0 && 2 * N < 64);
+  static_assert(STEPS % KG == 0 && (STAGES - 3) * N < 64);
   __shared__ __attribute__((aligned(256))) char lds[STAGES * STAGE > MEET ? STAGES * STAGE : MEET];
 
   const int head = blockIdx.x % p.kv_heads;
@@ -208,9 +115,8 @@ packed_attention_ring_kernel(PackedParams p) {
   bool none[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int load = wave * N + i;
-    const bool values = load >= STEPS * NC / 2;
-    const int slot = (values ? load - STEPS * NC / 2 : load) * 64 + lane, row = slot / NC;
+    const int load = min(wave * N + i, LOADS - 1), slot = load % (LOADS / 2) * 64 + lane, row = slot / NC;
+    const bool values = load >= LOADS / 2;
     const int c = L::Back(slot % NC, values ? L::WideTurn(row) : L::KTurn(row));
     off[i]  = row * (int)(values ? v_row : k_row) + c * 16;
     none[i] = c >= chunks;
@@ -221,13 +127,13 @@ packed_attention_ring_kernel(PackedParams p) {
     const char *k_tile = k_base + (int64_t)tile * KT * k_row, *v_tile = v_base + (int64_t)tile * KT * v_row;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int load = wave * N + i;
-      const bool values = load >= STEPS * NC / 2;
+      const int load = min(wave * N + i, LOADS - 1);
+      const bool values = load >= LOADS / 2;
       const char* from  = values ? v_tile : k_tile;
       if (chunks == NC && beyond <= 0) {
         CopyToLds16(from, off[i], to + load * 1024);
       } else {
-        const int row  = ((values ? load - STEPS * NC / 2 : load) * 64 + lane) / NC;
+        const int row  = (load % (LOADS / 2) * 64 + lane) / NC;
         const int back = max(row - (KT - 1 - beyond), 0) * (int)(values ? v_row : k_row);
         CopyToLds16(none[i] ? reinterpret_cast<const char*>(kZeros) : from + (int)(off[i] - back), to + load * 1024);
       }
@@ -270,6 +176,18 @@ packed_attention_ring_kernel(PackedParams p) {
     rows.Grow(top, ex);
   };
   auto values_of = [&](int n) { return keys_of(n) + STEPS * L::BYTES; };
+  if constexpr (WQ == 8) {
+    // without the branches of the loop below, where the code's length does not count
+#pragma unroll 1
+    for (; step < plain_steps; step += KG) {
+      rows.Grow(top, ex);
+      turn(step - kg + KG);
+      const typename Q::Probabilities mine = rows.Soften(s, ex);
+      s = rows.Scores(keys_of(step + KG), lane);
+      rows.Add(mine, values_of(step), lane);
+      top = Q::Top(s);
+    }
+  }
 #pragma unroll 1
   for (; step < tiles * STEPS; step += KG) {
     if (step < my_steps) open();
@@ -308,10 +226,140 @@ packed_attention_ring_kernel(PackedParams p) {
   rows.Store(out, p.d, 1.0f / sum, half);
 }
 
-template <typename T, int D, int WQ, int KG>
-void LaunchBlocks(PackedParams p, hipStream_t stream) {
-  p.tiles = (int)((int64_t)p.tokens * p.group.value / (32 * WQ)) + p.sequences + 1;
-  hipLaunchKernelGGL((packed_attention_kernel<T, D, WQ, KG>), dim3((unsigned)p.tiles * p.kv_heads), dim3(64 * WQ * KG), 0, stream, p);
+// The same with 16 x PT pairs a wavefront, for few pairs and for fp32: shorter chains of MFMAs and exponentials per step, and
+// twice the wavefronts, where latency counts.
+template <typename T, int D, int PT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, PT == 1 ? 2 : 1)
+packed_attention_few_kernel(PackedParams p) {
+  typedef FewPairs<T, D, PT> Q;
+  typedef Dense<T, D> L;
+  constexpr int NC = L::NC, STAGE = 2 * L::BYTES, STAGES = 4, LOADS = NC, N = (LOADS + WAVES - 1) / WAVES;  // the last is asked for again
+  __shared__ __attribute__((aligned(256))) char lds[STAGES * STAGE];
+  const int head = blockIdx.x % p.kv_heads;
+  const Found at = Find(p, blockIdx.x / p.kv_heads, 16 * PT * WAVES);
+  if (at.count == 0) {
+    ClearRest<T>(p, head, at.tile, at.more);
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int chunks = p.d * (int)sizeof(T) / 16, group = p.group.value, pairs = at.count * group;
+  const int pair0 = (at.tile * WAVES + wave) * 16 * PT;
+  const int first_query = p.group(min(pair0, pairs - 1));
+  const int last_query  = pair0 < pairs ? p.group(min(pair0 + 16 * PT - 1, pairs - 1)) : -1;
+  const int keys  = p.group(min((at.tile + 1) * WAVES * 16 * PT, pairs) - 1) + 1;
+  const int steps = (keys + 31) / 32, my_steps = __builtin_amdgcn_readfirstlane(last_query >= 0 ? last_query / 32 + 1 : 0);
+  const int plain_steps = __builtin_amdgcn_readfirstlane(last_query >= 0 ? (first_query + 1) / 32 : 0);
+
+  const int64_t k_row = p.k.row * sizeof(T), v_row = p.v.row * sizeof(T);
+  const char* k_base = HeadOf<T>(p.k, 0, head) + at.first * k_row;
+  const char* v_base = HeadOf<T>(p.v, 0, head) + at.first * v_row;
+  const unsigned lds_at = LdsAddress(lds);
+  unsigned off[N];
+  bool none[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int load = min(wave * N + i, LOADS - 1), slot = load % (LOADS / 2) * 64 + lane, row = slot / NC;
+    const bool values = load >= LOADS / 2;
+    const int c = L::Back(slot % NC, values ? L::RowTurn(row) : L::KTurn(row));
+    off[i]  = row * (int)(values ? v_row : k_row) + c * 16;
+    none[i] = c >= chunks;
+  }
+  auto request = [&](int step) {
+    const unsigned to = lds_at + step % STAGES * STAGE;
+    const int beyond  = at.first + (step + 1) * 32 - p.tokens;  // as in the other kernel
+    const char *k_tile = k_base + (int64_t)step * 32 * k_row, *v_tile = v_base + (int64_t)step * 32 * v_row;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int load = min(wave * N + i, LOADS - 1);
+      const bool values = load >= LOADS / 2;
+      const char* from  = values ? v_tile : k_tile;
+      if (chunks == NC && beyond <= 0) {
+        CopyToLds16(from, off[i], to + load * 1024);
+      } else {
+        const int row  = (load % (LOADS / 2) * 64 + lane) / NC;
+        const int back = max(row - (31 - beyond), 0) * (int)(values ? v_row : k_row);
+        CopyToLds16(none[i] ? reinterpret_cast<const char*>(kZeros) : from + (int)(off[i] - back), to + load * 1024);
+      }
+    }
+  };
+#pragma unroll 1
+  for (int i = 0; i < STAGES - 1 && i < steps; ++i) request(i);
+  Q rows;
+  int query[PT];
+#pragma unroll
+  for (int n = 0; n < PT; ++n) {
+    const int pair = min(pair0 + n * 16 + (lane & 15), pairs - 1);
+    query[n] = p.group(pair);
+    rows.Start(n, HeadOf<T>(p.q, 0, head * group + pair - query[n] * group) + (at.first + query[n]) * p.q.row * (int64_t)sizeof(T), chunks, lane,
+               p.scale);
+  }
+  const Exp<T> ex(p.scale);
+  WaitForAllBut<0>();  // the queries are the last that was asked for
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  // before a step's scores: its keys and values have landed, and everybody is done with those two before it
+  auto turn = [&](int step) {
+    if (step >= steps) return;
+    if (step + 1 < steps) {
+      WaitForAllBut<N>();
+    } else {
+      WaitForAllBut<0>();
+    }
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (step + STAGES - 2 < steps) request(step + STAGES - 2);
+  };
+  f32x4 s[PT][2];
+  unsigned word[PT];
+  auto keys_of   = [&](int n) { return lds + n % STAGES * STAGE; };
+  auto values_of = [&](int n) { return keys_of(n) + L::BYTES; };
+  int step = 0;
+  auto open = [&] {  // the step's scores are complete
+#pragma unroll
+    for (int n = 0; n < PT; ++n) {
+      word[n] = Below(query[n] + 1 - step * 32);
+      if (step >= plain_steps) Q::Mask(s[n], word[n], lane);
+    }
+  };
+  rows.Scores(s, keys_of(0), lane);
+#pragma unroll 1
+  for (; step < steps; ++step) {
+    if (step < my_steps) open();
+    turn(step + 1);
+    if (step >= my_steps) continue;
+    if (step >= plain_steps && Q::Unbounded(values_of(step), lane)) break;
+    f32x4 mine[PT][2];
+#pragma unroll
+    for (int n = 0; n < PT; ++n) {
+      rows.Soften(n, s[n], ex);
+      mine[n][0] = s[n][0], mine[n][1] = s[n][1];
+    }
+    rows.Scores(s, keys_of(step + 1), lane);
+    rows.Add(mine, values_of(step), lane);
+  }
+  // from the first step on whose values a mask alone does not keep out; it has been opened
+#pragma unroll 1
+  for (bool opened = true; step < steps; ++step, opened = false) {
+    if (!opened) {
+      if (step < my_steps) open();
+      turn(step + 1);
+    }
+    if (step >= my_steps) continue;
+#pragma unroll
+    for (int n = 0; n < PT; ++n) rows.Soften(n, s[n], ex);
+    rows.AddChosen(s, word, values_of(step), lane);
+    rows.Scores(s, keys_of(step + 1), lane);
+  }
+#pragma unroll
+  for (int n = 0; n < PT; ++n) {
+    float sum = rows.l[n] + __shfl_xor(rows.l[n], 16);
+    sum += __shfl_xor(sum, 32);
+    const int pair = pair0 + n * 16 + (lane & 15);
+    if (pair >= pairs) continue;
+    rows.Store(n, const_cast<char*>(HeadOf<T>(p.o, 0, head * group + pair - query[n] * group)) + (at.first + query[n]) * p.o.row * (int64_t)sizeof(T),
+               p.d, 1.0f / sum, lane);
+  }
 }
 
 template <typename T, int D, int WQ, int KG, int STEPS>
@@ -321,21 +369,20 @@ void LaunchRing(PackedParams p, hipStream_t stream) {
 }
 
 template <typename T, int D>
-void LaunchTiles(const PackedParams& p, hipStream_t stream) {
+void LaunchTiles(PackedParams p, hipStream_t stream) {
+  // Blocks of 128 pairs: how full the GPU is, whatever the lengths.  us, few | ring of 4 x 2 | 4 x 1 | 8 x 1 wavefronts, the
+  // choice in brackets.  bf16 32 heads over 8 x 128, one prompt of 64 [7.2] | 10.2 | 9.1 | 10.7, 256 [11.7] | 13.5 | 13.7 |
+  // 16.2, 1024 31.9 | [28.4] | 34.0 | 39.6, 2048 74.7 | [59.4] | 64.1 | 70.9, 4096 - | - | 150 | [142], 16384 - | - | 2100 |
+  // [1995]; 11 ragged prompts of 8126 330 | 264 | 205 | [200].  The wavefronts of a block wait for the one with the last
+  // queries: with one head a key head 256 queries apart, fp16 12 heads x 64, 8 x 1024 - | - | [33] | 37.
+  const int64_t blocks = (int64_t)p.tokens * p.group.value / 128 * p.kv_heads;
   if constexpr (sizeof(T) == 2) {
-    static const char* pick = getenv("PICK");
-    const int which = pick ? atoi(pick) : 0;
-    if (which == 0) return LaunchRing<T, D, 8, 1, 2>(p, stream);
-    if (which == 2) return LaunchRing<T, D, 4, 1, 1>(p, stream);
-    if (which == 3) return LaunchRing<T, D, 4, 2, 2>(p, stream);
+    if (blocks > 512) return p.group.value >= 4 ? LaunchRing<T, D, 8, 1, 2>(p, stream) : LaunchRing<T, D, 4, 1, 1>(p, stream);
+    if (blocks > 128) return LaunchRing<T, D, 4, 2, 2>(p, stream);
   }
-  // blocks of few pairs where there are few
-  const int64_t pairs = (int64_t)p.tokens * p.group.value * p.kv_heads;
-  if (pairs >= 256 * 128) {
-    LaunchBlocks<T, D, 4, 2>(p, stream);
-  } else {
-    LaunchBlocks<T, D, 1, 2>(p, stream);
-  }
+  constexpr int kPairs = 64;
+  p.tiles = (int)((int64_t)p.tokens * p.group.value / kPairs) + p.sequences + 1;
+  hipLaunchKernelGGL((packed_attention_few_kernel<T, D, 1, kPairs / 16>), dim3((unsigned)p.tiles * p.kv_heads), dim3(kPairs * 4), 0, stream, p);
 }
 
 template <typename T>
