@@ -333,6 +333,8 @@ cached_attention_few_kernel(CachedParams p) {
       }
     };
 
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) request_pages(min(tile0 + i, last));
     Q rows;
     unsigned long long seen[PT];
 #pragma unroll
@@ -341,8 +343,6 @@ cached_attention_few_kernel(CachedParams p) {
       rows.Start(n, HeadOf<T>(p.q, b, my_head) + token * p.q.row * (int64_t)sizeof(T), chunks, lane, p.scale);
       seen[n] = SeenBy(p, b, token);
     }
-#pragma unroll
-    for (int i = 0; i < STAGES; ++i) request_pages(min(tile0 + i, last));
     WaitForAllBut<0>();
 #pragma unroll
     for (int i = 0; i < STAGES; ++i) {
@@ -583,19 +583,23 @@ cached_attention_ring_kernel(CachedParams p) {
     auto keys_of = [&](int step) { return lds + step / STEPS % STAGES * STAGE + step % STEPS * L::BYTES; };
     auto values_of = [&](int step) { return keys_of(step) + STEPS * L::BYTES; };
 
-    request_pages(tile0);
-    request_pages(tile0 + 1);
+    // page numbers, parents and queries in one wait, then the rows
+#pragma unroll 1
+    for (int i = 0; i < STAGES; ++i) request_pages(tile0 + i);
+    Q rows;
+    rows.Start(HeadOf<T>(p.q, b, my_head) + token * p.q.row * (int64_t)sizeof(T), chunks, lane >> 5, p.scale);
+    const unsigned long long seen = SeenBy(p, b, token);
     WaitForAllBut<0>();
 #pragma unroll 1
     for (int i = 0; i < STAGES - 1 && tile0 + i < tile1; ++i) {
-      if (i == 2) WaitForAllBut<N + 1>();  // page numbers that were asked for before the first rows
-      request_pages(tile0 + i + 2);
+      if (i == 2) request_pages(tile0 + STAGES);
       request(tile0 + i);
     }
-    const unsigned long long seen = SeenBy(p, b, token);
-    Q rows;
-    rows.Start(HeadOf<T>(p.q, b, my_head) + token * p.q.row * (int64_t)sizeof(T), chunks, lane >> 5, p.scale);
-    WaitForAllBut<0>();
+    if (tile1 - tile0 > 2) {
+      WaitForAllBut<2 * N + 1>();
+    } else {
+      WaitForAllBut<0>();
+    }
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     // before the first step of a tile: it has landed, and everybody is done with the one before the last
@@ -672,12 +676,17 @@ cached_attention_ring_kernel(CachedParams p) {
 }
 
 // Units whose tiles several blocks had: a wavefront takes four registers of the lanes of TILE pairs, four consecutive elements
-// of d.  RUNS: of TILE pairs in a block's unit.
-template <typename T, int D, int TILE, int RUNS>
-__global__ void __launch_bounds__(64)
+// of d; SHARED: the eight of a block take the same ones, and a share of the parts each.  RUNS: of TILE pairs in a unit.
+template <typename T, int D, int TILE, int RUNS, bool SHARED>
+__global__ void __launch_bounds__(SHARED ? 512 : 256)
 cached_attention_join_kernel(CachedParams p, int keys_per_tile) {
   constexpr int GROUPS = 64 / TILE, QUADS = D / 4 / GROUPS, REGISTERS = QUADS * 4 + 2;  // lanes of one pair, fours of registers
-  const int lane = threadIdx.x, quad = blockIdx.x % QUADS, run = blockIdx.x / QUADS % RUNS, which = blockIdx.x / QUADS / RUNS;
+  constexpr int WAVES = SHARED ? 8 : 1;
+  __shared__ float shares[WAVES][6][64];
+  const int lane = threadIdx.x & 63, wave = SHARED ? threadIdx.x >> 6 : 0;
+  const int mine = SHARED ? blockIdx.x : blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int quad = mine % QUADS, run = mine / QUADS % RUNS, which = mine / QUADS / RUNS;
+  if (which >= p.batch * p.units) return;
   const int b = which / p.units, unit = which % p.units, pairs = p.tokens * p.group.value;
   const int pair0 = (unit / p.kv_heads * RUNS + run) * TILE, pair = pair0 + lane % TILE;
   if (pair0 >= pairs || quad * 4 * GROUPS >= p.d) return;
@@ -695,24 +704,54 @@ cached_attention_join_kernel(CachedParams p, int keys_per_tile) {
   const int64_t blocks = min((int64_t)p.blocks, total);
   const int block0 = (int)(((first + 1) * blocks - 1) / total), block1 = (int)(((first + tiles) * blocks - 1) / total);
   if (block0 == block1) return;  // that block has written the result
-  auto part = [&](int block) {
-    return p.parts + ((int64_t)(2 * block + (block == block0 ? 1 : 0)) * RUNS + run) * REGISTERS * 64 + lane;
-  };
   const Exp<T> ex(p.scale);
-  float top = -__builtin_inff();
-#pragma unroll 4
-  for (int i = block0; i <= block1; ++i) top = fmaxf(top, part(i)[(REGISTERS - 2) * 64]);
-  const float base = ex.Base(top);
-  float sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int i = block0; i <= block1; ++i) {
-    const float* from = part(i);
-    const float f     = ex(from[(REGISTERS - 2) * 64], base);
-    sum               = __builtin_fmaf(from[(REGISTERS - 1) * 64], f, sum);
+  float top = -__builtin_inff(), sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  bool token_is_none = false;
+  constexpr int AT_ONCE = 4;
+  for (int i0 = block0 + wave * AT_ONCE; i0 <= block1; i0 += WAVES * AT_ONCE) {
+    float m[AT_ONCE], l[AT_ONCE], v[AT_ONCE][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(from[(quad * 4 + e) * 64], f, o[e]);
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = min(i0 + u, block1);
+      const float* from = p.parts + ((int64_t)(2 * i + (i == block0 ? 1 : 0)) * RUNS + run) * REGISTERS * 64 + lane;
+      m[u] = from[(REGISTERS - 2) * 64], l[u] = from[(REGISTERS - 1) * 64];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[u][e] = from[(quad * 4 + e) * 64];
+    }
+    float grown = top;
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) grown = fmaxf(grown, m[u]);
+    const float base = ex.Base(grown), keep = ex(top, base);
+    top = grown, sum *= keep;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= keep;
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      if (i0 + u > block1) continue;
+      token_is_none |= l[u] < 0.0f;
+      const float f = ex(m[u], base);
+      sum           = __builtin_fmaf(l[u], f, sum);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(v[u][e], f, o[e]);
+    }
   }
-  const bool token_is_none = part(block0)[(REGISTERS - 1) * 64] < 0.0f;
+  if constexpr (SHARED) {
+    shares[wave][0][lane] = top, shares[wave][1][lane] = token_is_none ? -1.0f : sum;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) shares[wave][2 + e][lane] = o[e];
+    __syncthreads();
+    if (wave > 0) return;
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, shares[w][0][lane]);
+    const float base = ex.Base(top);
+    sum = 0.0f, o[0] = o[1] = o[2] = o[3] = 0.0f;
+    for (int w = 0; w < WAVES; ++w) {
+      const float f = ex(shares[w][0][lane], base);
+      token_is_none |= shares[w][1][lane] < 0.0f;
+      sum = __builtin_fmaf(shares[w][1][lane], f, sum);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(shares[w][2 + e][lane], f, o[e]);
+    }
+  }
   if (pair >= pairs) return;
   const int token = p.group(pair), my_head = unit % p.kv_heads * p.group.value + pair - token * p.group.value;
   const int at = (quad * GROUPS + lane / TILE) * 4;
@@ -746,8 +785,13 @@ int Divide(CachedParams& p, int tile, int runs, int keys_per_tile, hipStream_t s
 template <typename T, int D, int TILE, int RUNS>
 void LaunchJoin(const CachedParams& p, int keys_per_tile, hipStream_t stream) {
   if (p.blocks == 0) return;
-  hipLaunchKernelGGL((cached_attention_join_kernel<T, D, TILE, RUNS>), dim3((unsigned)(p.batch * p.units * RUNS * (D * TILE / 256))), dim3(64), 0,
-                     stream, p, keys_per_tile);
+  const int units = p.batch * p.units, wavefronts = units * RUNS * (D * TILE / 256);
+  if (p.blocks / units >= 8) {  // parts of a unit: four a wavefront at a time
+    hipLaunchKernelGGL((cached_attention_join_kernel<T, D, TILE, RUNS, true>), dim3((unsigned)wavefronts), dim3(512), 0, stream, p, keys_per_tile);
+  } else {
+    hipLaunchKernelGGL((cached_attention_join_kernel<T, D, TILE, RUNS, false>), dim3((unsigned)((wavefronts + 3) / 4)), dim3(256), 0, stream, p,
+                       keys_per_tile);
+  }
 }
 
 template <typename T, int D, int PT>
