@@ -796,8 +796,10 @@ void LaunchJoin(const CachedParams& p, int keys_per_tile, hipStream_t stream) {
 
 template <typename T, int D, int PT>
 void LaunchFew(CachedParams p, hipStream_t stream) {
-  // the buffers of eight (fp32 of more than 64 elements: four) wavefronts in 128 KiB of LDS
-  constexpr int kTile = 2 * Dense<T, D>::BYTES, kWaves = kTile > 16384 ? 4 : 8, kDeep = 128 * 1024 / kWaves / kTile;
+  // The buffers of eight wavefronts in 128 KiB of LDS; of four, which have twice the registers, where a tile, or the queries and
+  // sums of 32 pairs, need more than 256: 32 pairs a unit, 8 sequences of 2000 to 5000 bf16 rows, 8 key heads: d 128 40 us
+  // (eight: 57), d 96 37.4 us (39.3).
+  constexpr int kTile = 2 * Dense<T, D>::BYTES, kWaves = kTile * PT > 16384 ? 4 : 8, kDeep = 128 * 1024 / kWaves / kTile;
   constexpr int kStages = kDeep > 2 ? 2 : kDeep;
   const int blocks = Divide<D>(p, 16, PT, 32 * kWaves, stream);
   hipLaunchKernelGGL((cached_attention_few_kernel<T, D, PT, kWaves, kStages>), dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream, p);

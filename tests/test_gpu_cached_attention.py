@@ -118,6 +118,34 @@ def test_chains_and_trees(gpu, kind, layout, lengths, tokens, heads, kv_heads, d
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("lengths,tokens,heads,kv_heads,d,page", [
+    ([900, 3, 0, 4000], 1, 32, 1, 128, 16), ([700, 2500], 5, 4, 1, 96, 32), ([1300], 3, 18, 2, 128, 8), ([600, 33], 8, 8, 2, 64, 32),
+    ([2100, 9], 20, 2, 2, 120, 5), ([1800, 100], 16, 4, 1, 128, 16), ([2500, 64], 25, 8, 2, 128, 64), ([2000], 48, 4, 1, 128, 16),
+    ([1000, 640], 63, 4, 1, 96, 32), ([3000, 0, 1], 33, 12, 3, 112, 16)])
+def test_wide_heads_of_many_pairs(gpu, kind, lengths, tokens, heads, kv_heads, d, page):
+    Case(kind, lengths, tokens, heads, kv_heads, d, page).check()
+    Case(kind, lengths, tokens, heads, kv_heads, d, page, tree(np.random.default_rng(tokens), len(lengths), tokens, 0.1)).check()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("tokens,heads,d", [(1, 4, 128), (6, 8, 128), (9, 6, 96), (64, 2, 128)])
+def test_infinite_values_past_the_first_tiles(gpu, kind, tokens, heads, d):
+    """padding that holds an infinity, behind and among clean tiles: what attends to it is infinite, nothing else changes"""
+    parents = [[-1] * tokens, [-2] + [-1] * (tokens - 1)]
+    case = Case(kind, [1500, 700], tokens, heads, 2, d, 16, parents)
+    want, bound = case.reference()
+    case.data["v"][1, 0, :, 1] = rounded([np.inf], kind)[0][0]  # a token that is none
+    page = case.data["table"][0, 700 // 16]
+    case.data["v_pages"][page, 700 % 16, 1, 2] = rounded([np.inf], kind)[0][0]
+    got = case.run()
+    hit = np.zeros(want.shape, bool)
+    hit[0, :, heads // 2:, 2] = True
+    assert (as_float64(got, kind)[hit] == np.inf).all()
+    clean = np.where(hit, rounded(np.zeros(1), kind)[0][0], got)
+    assert_within(clean, np.where(hit, 0, want), np.where(hit, 1, bound), kind)
+
+
+@pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("tokens,heads", [(1, 2), (7, 4), (40, 4)])
 @pytest.mark.parametrize("length", [0, 50, 1200])
 def test_padding_among_the_tokens(gpu, kind, tokens, heads, length):
