@@ -1,6 +1,7 @@
 #include "hlir/lowering.h"
 
 #include <algorithm>
+#include <climits>
 #include <cstdlib>
 #include <functional>
 #include <limits>
@@ -1382,10 +1383,23 @@ ir::LoweredFuncRef OpLowerer::LowerLibraryCall(const Group& group) const {
       slots |= static_cast<uint32_t>(std::find(group.inputs.begin(), group.inputs.end(), n->inputs[s]) - group.inputs.begin()) << (4 * s);
     return static_cast<int>(slots);
   };
-  // rows of an attention are moved 16 bytes at a time
+  auto check_numel = [&](const NodeData* x) {
+    int64_t numel = 1;
+    for (int extent : x->shape) {
+      numel *= extent;
+      CINN_CHECK(numel < INT_MAX) << op << ": a tensor of 2^31 elements or more";
+    }
+  };
+  // rows of an attention are moved 16 bytes at a time, tiles of them with offsets of 32 bits
   auto check_rows = [&] {
     const NodeData* q = n->inputs[0];
-    CINN_CHECK_EQ(q->shape.back() * q->dtype.bytes() % 16, 0) << op << ": heads of " << q->shape.back() << " elements are no whole number of 16-byte chunks";
+    const int64_t row = int64_t{q->shape.back()} * q->dtype.bytes();
+    CINN_CHECK_EQ(row % 16, 0) << op << ": heads of " << q->shape.back() << " elements are no whole number of 16-byte chunks";
+    for (int i = 0; i < 3; ++i) {
+      const auto& shape = n->inputs[i]->shape;
+      check_numel(n->inputs[i]);
+      CINN_CHECK(row * shape[shape.size() - 2] <= (1 << 25)) << op << ": more than 32 MiB a row";
+    }
   };
   // q, k and v: how many heads the tensor has and the first one in use
   auto push_attention_heads = [&] {
@@ -1648,8 +1662,10 @@ ir::LoweredFuncRef OpLowerer::LowerLibraryCall(const Group& group) const {
     const auto& q  = n->inputs[0]->shape;
     const int all  = n->outputs[0]->shape[1];
     check_rows();
+    const int kv_heads = AttentionKvHeads(n->inputs[1]->shape[1], n->attrs), sequences = n->inputs[3]->shape[0] - 1;
+    CINN_CHECK((int64_t{q[0]} * (all / kv_heads) / 32 + sequences + 1) * kv_heads < (1 << 23)) << op << ": too many rows or sequences";
     args.push_back(Expr(GetAttr<float>(n->attrs, "scale", 1.0f)));
-    push_ints({q[0], n->inputs[3]->shape[0] - 1, all, AttentionKvHeads(n->inputs[1]->shape[1], n->attrs), q[2], operand_slots()});
+    push_ints({q[0], sequences, all, kv_heads, q[2], operand_slots()});
     push_attention_heads();
   } else if (op == "cached_attention") {
     api               = "cinn_call_hip_cached_attention";
@@ -1657,6 +1673,9 @@ ir::LoweredFuncRef OpLowerer::LowerLibraryCall(const Group& group) const {
     const auto& pages = n->inputs[3]->shape;
     const bool by_row = GetAttr<std::string>(n->attrs, "page_layout", "row_head") == "row_head";
     check_rows();
+    CINN_CHECK(int64_t{q[0]} * q[1] * n->outputs[0]->shape[2] < (1 << 22)) << op << ": too many rows";
+    CINN_CHECK(int64_t{q[0]} * n->inputs[5]->shape[1] < INT_MAX) << op << ": a table of 2^31 elements or more";
+    CINN_CHECK(ShapeNumel(pages) < (int64_t{1} << 40)) << op << ": pages of 2^40 elements or more";
     args.push_back(Expr(GetAttr<float>(n->attrs, "scale", 1.0f)));
     push_ints({q[0], q[1], n->outputs[0]->shape[2], AttentionKvHeads(n->inputs[1]->shape[2], n->attrs), q[3]});
     push_ints({pages[0], by_row ? pages[1] : pages[2], by_row ? 0 : 1, n->inputs[5]->shape[1]});
@@ -1667,6 +1686,7 @@ ir::LoweredFuncRef OpLowerer::LowerLibraryCall(const Group& group) const {
     const auto& x = n->inputs[0]->shape;
     const auto& y = n->outputs[0]->shape;
     const int d = x.back(), total_heads = x[x.size() - 2], rotary_dim = GetAttr<int>(n->attrs, "rotary_dim", 0);
+    check_numel(n->inputs[0]);
     push_ints({static_cast<int>(ShapeNumel(x) / d / total_heads), y[y.size() - 2], total_heads, d, rotary_dim > 0 ? rotary_dim : d});
     push_ints({GetAttr<bool>(n->attrs, "interleaved", false) ? 1 : 0, GetAttr<bool>(n->attrs, "transposed", false) ? 1 : 0});
     auto push_double = [&](const char* name, double dflt) {

@@ -875,8 +875,10 @@ extern "C" void cinn_call_hip_cached_attention(void* v_args, int num_args, float
   const bool f16 = out->type.code == cinn_type_float && out->type.bits == 16;
   CINN_RT_CHECK(f32 || f16 || (out->type.code == cinn_type_bfloat && out->type.bits == 16), "cached_attention: fp16 / bf16 / fp32 only");
   CINN_RT_CHECK(d % (f32 ? 4 : 8) == 0, "cached_attention: rows of %d elements are no whole number of 16-byte chunks", d);
-  CINN_RT_CHECK((int64_t)batch * tokens * d * std::max(std::max(q_heads, k_heads), v_heads) < INT_MAX && (int64_t)batch * columns < INT_MAX &&
-                    (int64_t)pages * page_rows * kv_heads * d < ((int64_t)1 << 40),
+  const int64_t row = (int64_t)d * std::max(std::max(q_heads, k_heads), v_heads);
+  CINN_RT_CHECK(row * (f32 ? 4 : 2) <= 1 << 25, "cached_attention: rows of more than 32 MiB");  // a load's offsets have 32 bits
+  CINN_RT_CHECK((int64_t)batch * heads * tokens < 1 << 22, "cached_attention: too many rows");  // blocks of up to 512 threads
+  CINN_RT_CHECK((int64_t)batch * tokens * row < INT_MAX && (int64_t)batch * columns < INT_MAX && (int64_t)pages * page_rows * kv_heads * d < (int64_t)1 << 40,
                 "cached_attention: tensor too large");
   auto input = [&](int slot) {
     const int at = ((unsigned)operands >> (4 * slot)) & 15;
@@ -886,6 +888,7 @@ extern "C" void cinn_call_hip_cached_attention(void* v_args, int num_args, float
   auto typed = [&](int slot) {
     const cinn_buffer_t* b = input(slot);
     CINN_RT_CHECK(b->type.code == out->type.code && b->type.bits == out->type.bits, "cached_attention: operands of different types");
+    CINN_RT_CHECK(reinterpret_cast<uintptr_t>(b->memory) % 16 == 0, "cached_attention: operand %d is not aligned to 16 bytes", slot);
     return b->memory;
   };
   auto whole = [&](int slot) {
@@ -906,7 +909,6 @@ extern "C" void cinn_call_hip_cached_attention(void* v_args, int num_args, float
   p.table = whole(5), p.lengths = whole(6), p.parents = ((unsigned)operands >> 28) == 15 ? nullptr : whole(7);
   p.batch = batch, p.tokens = tokens, p.kv_heads = kv_heads, p.d = d, p.pages = pages, p.columns = columns;
   p.page_rows = Divisor(page_rows), p.group = Divisor(heads / kv_heads), p.scale = scale;
-  CINN_RT_CHECK((int64_t)batch * heads * tokens < (1 << 24), "cached_attention: too many rows");
   auto s = static_cast<hipStream_t>(stream);
   if (f32) {
     Launch<float>(p, s);

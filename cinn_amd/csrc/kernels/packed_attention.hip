@@ -423,7 +423,9 @@ extern "C" void cinn_call_hip_packed_attention(void* v_args, int num_args, float
   const bool f16 = out->type.code == cinn_type_float && out->type.bits == 16;
   CINN_RT_CHECK(f32 || f16 || (out->type.code == cinn_type_bfloat && out->type.bits == 16), "packed_attention: fp16 / bf16 / fp32 only");
   CINN_RT_CHECK(d % (f32 ? 4 : 8) == 0, "packed_attention: rows of %d elements are no whole number of 16-byte chunks", d);
-  CINN_RT_CHECK((int64_t)tokens * d * std::max(std::max(q_heads, k_heads), v_heads) < INT_MAX, "packed_attention: tensor too large");
+  const int64_t row = (int64_t)d * std::max(std::max(q_heads, k_heads), v_heads);
+  CINN_RT_CHECK(tokens * row < INT_MAX, "packed_attention: tensor too large");
+  CINN_RT_CHECK(row * (f32 ? 4 : 2) <= 1 << 25, "packed_attention: rows of more than 32 MiB");  // a tile's offsets have 32 bits
   auto input = [&](int slot) {
     const int at = (operands >> (4 * slot)) & 15;
     CINN_RT_CHECK(at < num_args - 1, "packed_attention: operand %d is argument %d of %d", slot, at, num_args);
@@ -432,6 +434,7 @@ extern "C" void cinn_call_hip_packed_attention(void* v_args, int num_args, float
   auto rows = [&](int slot, int total, int first) {
     const cinn_buffer_t* b = input(slot);
     CINN_RT_CHECK(b->type.code == out->type.code && b->type.bits == out->type.bits, "packed_attention: operands of different types");
+    CINN_RT_CHECK(reinterpret_cast<uintptr_t>(b->memory) % 16 == 0, "packed_attention: operand %d is not aligned to 16 bytes", slot);
     return Rows{b->memory + (int64_t)first * d * (f32 ? 4 : 2), 0, d, (int64_t)total * d};
   };
   PackedParams p;
@@ -441,7 +444,8 @@ extern "C" void cinn_call_hip_packed_attention(void* v_args, int num_args, float
   CINN_RT_CHECK(offsets->type.code == cinn_type_int && offsets->type.bits == 32, "packed_attention: offsets are int32");
   p.offsets = reinterpret_cast<const int*>(offsets->memory);
   p.sequences = sequences, p.tokens = tokens, p.kv_heads = kv_heads, p.d = d, p.tiles = 0, p.group = Divisor(heads / kv_heads), p.scale = scale;
-  CINN_RT_CHECK(((int64_t)tokens * p.group.value / 32 + sequences + 1) * kv_heads < INT_MAX, "packed_attention: too many tiles");
+  // blocks of up to 512 threads
+  CINN_RT_CHECK(((int64_t)tokens * p.group.value / 32 + sequences + 1) * kv_heads < 1 << 23, "packed_attention: too many rows or sequences");
   auto s = static_cast<hipStream_t>(stream);
   if (f32) {
     Launch<float>(p, s);

@@ -288,8 +288,9 @@ void cinn_call_hip_attention(void* v_args, int num_args, float scale, int batch,
  * [tokens][heads][d].  Rows before offsets[0] and from offsets[sequences] on belong to no sequence: out is zero there.
  * Keys and values that a row does not attend to, infinities and NaN among them, do not count.  offsets: int32
  * [sequences + 1], in order, read on the GPU; with offsets out of order or range results are unspecified, accesses in
- * bounds.  fp16 / bf16 / fp32; d at most 128, a multiple of 16 bytes.  operands: four bits for each of the slots q, k, v,
- * offsets, which input it is; v_args = {inputs..., out}.  No counterpart in the reference. */
+ * bounds.  fp16 / bf16 / fp32; d at most 128, a multiple of 16 bytes; q, k and v aligned to 16 bytes, out apart from them;
+ * fewer than 2^31 elements a tensor, at most 32 MiB a row.  operands: four bits for each of the slots q, k, v, offsets, which
+ * input it is; v_args = {inputs..., out}.  No counterpart in the reference. */
 void cinn_call_hip_packed_attention(void* v_args, int num_args, float scale, int tokens, int sequences, int heads, int kv_heads,
                                     int d, int operands, int q_heads, int q_head, int k_heads, int k_head, int v_heads, int v_head,
                                     void* stream);
@@ -302,9 +303,10 @@ void cinn_call_hip_packed_attention(void* v_args, int num_args, float scale, int
  * [kv_heads][d] (page_layout 0) or [pages][kv_heads][page_rows][d] (1); row r of sequence b lies in page table[b][r /
  * page_rows] of table [batch][columns].  lengths are taken between 0 and columns * page_rows; a page number out of range
  * holds no rows.  table, lengths and parents are int32, read on the GPU.  fp16 / bf16 / fp32; d at most 128, a multiple of 16
- * bytes.  operands: four bits for each of the slots q, k, v, k pages, v pages, table, lengths, parents, which input it is;
+ * bytes; alignment and sizes as in cinn_call_hip_packed_attention, batch * tokens * heads below 2^22.  operands: four bits for each of the slots q, k, v, k pages, v pages, table, lengths, parents, which input it is;
  * v_args = {inputs..., out}.  Long caches are divided over blocks by way of the stream's split-K scratch
- * (cinn_hip_scratch_reserve); under capture with too little of it, over fewer.  No counterpart in the reference. */
+ * (cinn_hip_scratch_reserve); under capture with too little of it, over fewer.  A replayed graph uses the scratch of the
+ * stream that it was captured on, and threads that share a stream take turns.  No counterpart in the reference. */
 void cinn_call_hip_cached_attention(void* v_args, int num_args, float scale, int batch, int tokens, int heads, int kv_heads, int d,
                                     int pages, int page_rows, int page_layout, int columns, int operands, int q_heads, int q_head,
                                     int k_heads, int k_head, int v_heads, int v_head, void* stream);

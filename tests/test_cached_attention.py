@@ -37,6 +37,18 @@ def test_rows_of_odd_bytes_are_refused():
         compile_only(b, [o])
 
 
+@pytest.mark.parametrize("case", [
+    dict(q=(3, 5, 1 << 18, 128), k=(3, 5, 2, 128), v=(3, 5, 2, 128), k_pages=(7, 16, 2, 128)),
+    dict(q=(3, 5, 2, 128), k=(3, 5, 1 << 18, 128), v=(3, 5, 2, 128), k_pages=(7, 16, 2, 128), kv_heads=2),
+    dict(q=(1 << 17, 1, 32, 64), k=(1 << 17, 1, 2, 64), v=(1 << 17, 1, 2, 64), table=(1 << 17, 4), lengths=(1 << 17,), parents=None),
+    dict(q=(1 << 16, 1, 8, 64), k=(1 << 16, 1, 2, 64), v=(1 << 16, 1, 2, 64), table=(1 << 16, 1 << 15), lengths=(1 << 16,), parents=None),
+    dict(k_pages=(1 << 30, 16, 2, 64))])
+def test_sizes_that_its_offsets_do_not_hold_are_refused(case):
+    b, o = made(**case)
+    with pytest.raises(_lib.CinnError, match="32 MiB|2\\^31|2\\^40|too many"):
+        compile_only(b, [o])
+
+
 @pytest.mark.parametrize("case", [dict(), dict(parents=None), dict(k_pages=(7, 2, 16, 64), page_layout="head_row"),
                                   dict(heads=4, q_head=2, kv_heads=2, v_head=0), dict(k_pages=(1, 1, 2, 64), table=(3, 1))])
 def test_one_call(case):

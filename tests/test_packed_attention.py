@@ -34,6 +34,15 @@ def test_rows_of_odd_bytes_are_refused(kind, d):
         compile_only(b, [o])
 
 
+@pytest.mark.parametrize("case", [
+    dict(q=(4, 1 << 18, 128), k=(4, 1, 128), v=(4, 1, 128)), dict(q=(4, 1, 128), k=(4, 1 << 18, 128), v=(4, 1, 128), kv_heads=1),
+    dict(q=(1 << 22, 8, 128), k=(1 << 22, 1, 128), v=(1 << 22, 1, 128)), dict(offsets=(1 << 23,)), dict(q=(1 << 28, 1, 8), k=(1 << 28, 1, 8), v=(1 << 28, 1, 8))])
+def test_sizes_that_its_offsets_do_not_hold_are_refused(case):
+    b, o = made(**case)
+    with pytest.raises(_lib.CinnError, match="32 MiB|2\\^31|too many"):
+        compile_only(b, [o])
+
+
 @pytest.mark.parametrize("case", [dict(), dict(heads=4, kv_heads=1, q_head=3, k_head=1, v_head=0), dict(k_head=1, v_head=1), dict(offsets=(2,))])
 def test_one_call(case):
     b, o = made(**case)

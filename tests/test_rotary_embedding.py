@@ -25,6 +25,12 @@ def test_refused(case):
         made(**case)
 
 
+def test_tensors_of_many_elements_are_refused():
+    b, y = made((1 << 20, 32, 128), (1 << 20,), heads=1)
+    with pytest.raises(_lib.CinnError, match="2\\^31"):
+        compile_only(b, [y])
+
+
 @pytest.mark.parametrize("case", [dict(), dict(x=(4, 3, 600), rotary_dim=512), dict(x=(2, 2, 3, 33), positions=(2, 2), rotary_dim=32),
                                   dict(x=(3, 32), positions=(1,)), dict(heads=2, p_type=Int(64))])
 def test_one_call(case):
