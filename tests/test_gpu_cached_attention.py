@@ -11,6 +11,7 @@ from cinn_amd.common import DefaultAMDGPUTarget, Int
 from cinn_amd.frontend import Computation, NetBuilder
 
 from helpers import run
+from test_gpu_gradient_capture import fresh_stream, replays
 from typed_inputs import TYPES, as_float64, assert_within, attend, dtype, normal, rounded
 
 pytestmark = pytest.mark.gpu
@@ -268,3 +269,23 @@ def test_two_programs_on_two_streams(gpu):
     runtime.synchronize()
     for (comp, o), want in zip(comps, alone):
         assert np.array_equal(comp.get_tensor(o.id).numpy().view(np.uint16), want.view(np.uint16))
+
+
+@pytest.mark.parametrize("kind", ["float16", "float32"])
+@pytest.mark.parametrize("tokens,heads", [(1, 4), (12, 4), (64, 4)])
+def test_captured_without_an_eager_run(gpu, kind, tokens, heads):
+    """called first while its stream is captured, with no scratch to divide a long cache over blocks: one block each"""
+    case = Case(kind, [1700, 0, 300], tokens, heads, 2, 64, 16)
+    lib = _lib.load()
+    lib.cinn_call_hip_cached_attention.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_float] + [ctypes.c_int] * 16 + [ctypes.c_void_p]
+    want, bound = case.reference()
+    clear = np.full(want.shape, 7, kind)
+    out = runtime.DeviceBuffer.from_numpy(clear)
+    inputs = [runtime.DeviceBuffer.from_numpy(x) for x in case.data.values()]
+    pods = runtime.pod_args(inputs + [out])
+    stream = fresh_stream(lib, 0)
+    pages, columns = case.data["k_pages"].shape[0], case.data["table"].shape[1]
+    args = [64 ** -0.5, 3, tokens, heads, 2, 64, pages, 16, 0, columns, (0x06543210 | 15 << 28) - (1 << 32), heads, 0, 2, 0, 2, 0]
+    for got in replays(stream, lambda: lib.cinn_call_hip_cached_attention(pods, 8, *args, stream.handle), out, clear):
+        assert_within(got.numpy(), want, bound, kind)
+        case.check()
