@@ -560,7 +560,10 @@ __device__ __forceinline__ void CopyToLds16(const void* base, unsigned off, unsi
   const uint64_t at = (uint64_t)base;
   base = (const void*)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(at >> 32)) << 32 |
                        (unsigned)__builtin_amdgcn_readfirstlane((unsigned)at));
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(off), "s"(base) : "memory");
+  // by way of a scalar copy: a vector memory instruction may not read a scalar register right behind a vector instruction, a
+  // readlane or a reload among them, that wrote it
+  uint64_t copy;
+  asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0" : "=&s"(copy) : "s"(to), "v"(off), "s"(base) : "memory");
 }
 __device__ __forceinline__ void CopyToLds4(const void* from, unsigned to) {
   to = __builtin_amdgcn_readfirstlane(to);

@@ -46,11 +46,17 @@ __device__ __forceinline__ int LengthOf(const CachedParams& p, int b) {
 // blocks with many short sequences have fewer of them.
 constexpr int kEmpty = 1;
 
-// Where item `item` of the list of all tiles lies: its sequence, that one's rows in the cache and first item.  With item < 0
-// only the items are counted.  By every wavefront for itself, 64 sequences at a time.
+// what lane `lane` has, in scalar registers
+__device__ __forceinline__ int64_t OfLane(int64_t v, int lane) {
+  return (int64_t)((uint64_t)(unsigned)__builtin_amdgcn_readlane((unsigned)((uint64_t)v >> 32), lane) << 32 |
+                   (unsigned)__builtin_amdgcn_readlane((unsigned)v, lane));
+}
+
+// Which sequence item `item` of the list of all tiles belongs to, and that one's first item; with item < 0 how many items there
+// are.  By every wavefront for itself, 64 sequences at a time.
 struct Place {
-  int b, length;
-  int64_t first, count;
+  int b;
+  int64_t first;
 };
 __device__ __forceinline__ Place Find(const CachedParams& p, int64_t item, int keys_per_tile) {
   const int lane = threadIdx.x & 63;
@@ -67,12 +73,49 @@ __device__ __forceinline__ Place Find(const CachedParams& p, int64_t item, int k
     const unsigned long long behind = item < 0 ? 0 : __ballot(before + sum > item);
     if (behind) {
       const int at = __ffsll(behind) - 1;
-      return {b0 + at, __shfl(length, at), before + __shfl((long long)(sum - mine), at), __shfl((long long)mine, at)};
+      return {b0 + at, before + OfLane(sum - mine, at)};
     }
-    before += __shfl((long long)sum, 63);
+    before += OfLane(sum, 63);
   }
-  return {0, 0, 0, before};
+  return {0, before};
 }
+
+// A block's share of the list: runs of tiles tile0 .. tile1 - 1 of the `tiles` of a unit, one after the other.
+struct Share {
+  int b, unit, length, tiles, tile0, tile1;
+  int next, item;  // the unit and the item of it that the next run begins with
+  int64_t left;    // items
+  __device__ __forceinline__ Share(const CachedParams& p, int keys_per_tile) {
+    if (p.blocks > 0) {
+      // no more blocks than items: every block that the second kernel looks at has some
+      const int64_t total = Find(p, -1, keys_per_tile).first, blocks = min((int64_t)p.blocks, total);
+      left = 0;
+      if (blockIdx.x >= blocks) return;
+      const int64_t at  = total * blockIdx.x / blocks;
+      const Place place = Find(p, at, keys_per_tile);
+      left = total * (blockIdx.x + 1) / blocks - at;
+      Open(p, place.b, keys_per_tile);
+      next = (int)((at - place.first) / (tiles + kEmpty));
+      item = (int)(at - place.first - (int64_t)next * (tiles + kEmpty));
+    } else {
+      Open(p, blockIdx.x / p.units, keys_per_tile);
+      next = blockIdx.x % p.units, item = 0, left = tiles + kEmpty;
+    }
+  }
+  __device__ __forceinline__ void Open(const CachedParams& p, int sequence, int keys_per_tile) {
+    b = sequence, length = LengthOf(p, sequence), tiles = (length + p.tokens + keys_per_tile - 1) / keys_per_tile;
+  }
+  __device__ __forceinline__ bool Next(const CachedParams& p, int keys_per_tile) {
+    while (left > 0) {
+      if (next == p.units) Open(p, b + 1, keys_per_tile), next = 0;
+      const int end = (int)min((int64_t)tiles + kEmpty, item + left);
+      tile0 = max(item - kEmpty, 0), tile1 = end - kEmpty, unit = next++;
+      left -= end - item, item = 0;
+      if (tile0 < tile1) return true;
+    }
+    return false;
+  }
+};
 
 // which new tokens token `token` (of this lane) attends to, itself among them; none: it is no token
 __device__ __forceinline__ unsigned long long SeenBy(const CachedParams& p, int b, int token) {
@@ -123,28 +166,11 @@ cached_attention_kernel(CachedParams p) {
   const int chunks = p.d * (int)sizeof(T) / 16, pairs = p.tokens * p.group.value;
   const Exp<T> ex(p.scale);
 
-  int64_t at, end;  // this block's items
-  Place place;
-  if (p.blocks > 0) {
-    // no more blocks than items: every block that the second kernel looks at has some
-    const int64_t total = Find(p, -1, KT).count, blocks = min((int64_t)p.blocks, total);
-    if (blockIdx.x >= blocks) return;
-    at = total * blockIdx.x / blocks, end = total * (blockIdx.x + 1) / blocks;
-    place = Find(p, at, KT);
-  } else {
-    const int b = blockIdx.x / p.units, length = LengthOf(p, b), tiles = (length + p.tokens + KT - 1) / KT;
-    at = (int64_t)(blockIdx.x % p.units) * (tiles + kEmpty), end = at + tiles + kEmpty;
-    place = {b, length, 0, (int64_t)(tiles + kEmpty) * p.units};
-  }
+  Share share(p, KT);
 #pragma unroll 1
-  while (at < end) {
-    if (at >= place.first + place.count) place = Find(p, at, KT);
-    const int b = place.b, length = place.length, keys = length + p.tokens, tiles = (keys + KT - 1) / KT;
-    const int64_t inside = at - place.first, items = tiles + kEmpty;
-    const int unit = (int)(inside / items), item0 = (int)(inside - unit * items), item1 = (int)min(items, item0 + end - at);
-    const int tile0 = max(item0 - kEmpty, 0), tile1 = item1 - kEmpty;
-    at += item1 - item0;
-    if (tile0 >= tile1) continue;
+  while (share.Next(p, KT)) {
+    const int b = share.b, unit = share.unit, length = share.length, keys = length + p.tokens;
+    const int tiles = share.tiles, tile0 = share.tile0, tile1 = share.tile1;
     const int head = unit % p.kv_heads, pair0 = (unit / p.kv_heads * WQ + wq) * 32;
     const int pair = min(pair0 + (lane & 31), pairs - 1), token = p.group(pair), my_head = head * p.group.value + pair - token * p.group.value;
     const unsigned long long seen = SeenBy(p, b, token);
@@ -254,27 +280,11 @@ cached_attention_few_kernel(CachedParams p) {
     v_off[j] = lane / NC * row_bytes + L::Back(lane % NC, L::RowTurn(j * RPL + lane / NC)) * 16;
   }
 
-  int64_t at, end;  // this block's items
-  Place place;
-  if (p.blocks > 0) {
-    const int64_t total = Find(p, -1, KT).count, blocks = min((int64_t)p.blocks, total);
-    if (blockIdx.x >= blocks) return;
-    at = total * blockIdx.x / blocks, end = total * (blockIdx.x + 1) / blocks;
-    place = Find(p, at, KT);
-  } else {
-    const int b = blockIdx.x / p.units, length = LengthOf(p, b), tiles = (length + p.tokens + KT - 1) / KT;
-    at = (int64_t)(blockIdx.x % p.units) * (tiles + kEmpty), end = at + tiles + kEmpty;
-    place = {b, length, 0, (int64_t)(tiles + kEmpty) * p.units};
-  }
+  Share share(p, KT);
 #pragma unroll 1
-  while (at < end) {
-    if (at >= place.first + place.count) place = Find(p, at, KT);
-    const int b = place.b, length = place.length, keys = length + p.tokens, tiles = (keys + KT - 1) / KT;
-    const int64_t inside = at - place.first, items = tiles + kEmpty;
-    const int head = (int)(inside / items), item0 = (int)(inside - head * items), item1 = (int)min(items, item0 + end - at);
-    const int tile0 = max(item0 - kEmpty, 0), tile1 = item1 - kEmpty, last = tile1 - 1;
-    at += item1 - item0;
-    if (tile0 >= tile1) continue;
+  while (share.Next(p, KT)) {
+    const int b = share.b, head = share.unit, length = share.length, keys = length + p.tokens;
+    const int tiles = share.tiles, tile0 = share.tile0, tile1 = share.tile1, last = tile1 - 1;
     const char* k_new = HeadOf<T>(p.k, b, head);
     const char* v_new = HeadOf<T>(p.v, b, head);
     const int* table  = p.table + (int64_t)b * p.columns;
@@ -509,29 +519,11 @@ cached_attention_ring_kernel(CachedParams p) {
     lane_off[i]    = lane / NC * (int)(p.row * sizeof(T)) + L::Back(slot % NC, load >= LOADS / 2 ? L::WideTurn(row) : L::KTurn(row)) * 16;
   }
 
-  int64_t at, end;  // this block's items
-  Place place;
-  if (p.blocks > 0) {
-    const int64_t total = Find(p, -1, KT).count, blocks = min((int64_t)p.blocks, total);
-    if (blockIdx.x >= blocks) return;
-    at = total * blockIdx.x / blocks, end = total * (blockIdx.x + 1) / blocks;
-    place = Find(p, at, KT);
-  } else {
-    const int b = blockIdx.x / p.units, length = LengthOf(p, b), tiles = (length + p.tokens + KT - 1) / KT;
-    at = (int64_t)(blockIdx.x % p.units) * (tiles + kEmpty), end = at + tiles + kEmpty;
-    place = {b, length, 0, (int64_t)(tiles + kEmpty) * p.units};
-  }
+  Share share(p, KT);
 #pragma unroll 1
-  while (at < end) {
-    if (at >= place.first + place.count) place = Find(p, at, KT);
-    const int b = __builtin_amdgcn_readfirstlane(place.b), length = __builtin_amdgcn_readfirstlane(place.length);
-    const int keys = length + p.tokens, tiles = (keys + KT - 1) / KT;
-    const int64_t inside = at - place.first, items = tiles + kEmpty;
-    const int unit = __builtin_amdgcn_readfirstlane((int)(inside / items)), item0 = __builtin_amdgcn_readfirstlane((int)(inside - unit * items));
-    const int item1 = __builtin_amdgcn_readfirstlane((int)min(items, item0 + end - at));
-    const int tile0 = max(item0 - kEmpty, 0), tile1 = item1 - kEmpty;
-    at += item1 - item0;
-    if (tile0 >= tile1) continue;
+  while (share.Next(p, KT)) {
+    const int b = share.b, unit = share.unit, length = share.length, keys = length + p.tokens;
+    const int tiles = share.tiles, tile0 = share.tile0, tile1 = share.tile1;
     const int head = unit % p.kv_heads, pair0 = (unit / p.kv_heads * WQ + wq) * 32;
     const int pair = min(pair0 + (lane & 31), pairs - 1), token = p.group(pair), my_head = head * p.group.value + pair - token * p.group.value;
     const char* k_new = HeadOf<T>(p.k, b, head);
