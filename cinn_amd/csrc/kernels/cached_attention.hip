@@ -43,7 +43,8 @@ __device__ __forceinline__ int LengthOf(const CachedParams& p, int b) {
 }
 
 // What a block's change of units costs beside its tiles, in tiles: every unit has that many empty items in front, so that the
-// blocks with many short sequences have fewer of them.
+// blocks with many short sequences have fewer of them.  us without | with one: bf16 48 sequences of 100 to 16000 rows, 32 heads
+// over 8 x 128, 178 | 153, of 100 to 4000 58 | 45, 8 trees of 48 tokens 68 | 66; with two or three 159 and 161 instead of 157.
 constexpr int kEmpty = 1;
 
 // what lane `lane` has, in scalar registers
@@ -249,15 +250,19 @@ cached_attention_kernel(CachedParams p) {
   }
 }
 
-// At most 16 PT pairs: a wavefront streams 32 keys of every tile through buffers of its own in LDS, STAGES deep for keys and
-// for values, that loads fill directly, and meets the others at the end of a unit only.  The next keys are requested as soon
-// as the scores are there, the next values when they are summed.  Which pages the rows lie in comes the same way, STAGES
-// tiles ahead of them: every wavefront's loads land in order, so that one count tells what has.
+// At most 16 PT pairs, bound by the cache's bytes: a wavefront streams 32 keys of every tile through buffers of its own in LDS,
+// STAGES deep for keys and for values, that loads fill directly, and meets the others at the end of a unit only.  The next keys
+// are requested as soon as the scores are there, the next values when they are summed.  Which pages the rows lie in comes the same way, STAGES
+// tiles ahead of them: every wavefront's loads land in order, so that one count tells what has.  Measured: 48 sequences of 100 to
+// 16000 bf16 rows, 32 heads over 8 x 128, 154 us, 5.0 TB/s; one of 100003 fp32 rows, 16 over 4 x 96, 72 us, 4.3 TB/s (96 KiB of
+// loads in flight on a CU, less while their scores are taken); 8 of 511 fp16 rows, 12 x 64, 7.3 us, of which a launch is 4.
+// Wavefronts with tiles shared through registers took 567, 345 and 23.
 template <typename T, int D, int PT, int WAVES, int STAGES>
 __global__ void __launch_bounds__(64 * WAVES, (WAVES + 3) / 4)
 cached_attention_few_kernel(CachedParams p) {
   typedef FewPairs<T, D, PT> Q;
   typedef Dense<T, D> L;
+  static_assert(STAGES == 1 || STAGES == 2);
   constexpr int KT = 32 * WAVES, NC = L::NC, N = NC / 2;  // N: loads for a tile of keys or of values
   constexpr int RPL = 64 / NC;                            // rows per load, where that is a whole number
   constexpr int IDS = 4 * STAGES, IDS_AT = STAGES * 2 * L::BYTES, ROWS_AT = IDS_AT + IDS * 256, WAVE = ROWS_AT + STAGES * 32 * 16;
@@ -370,10 +375,6 @@ cached_attention_few_kernel(CachedParams p) {
       const char* cur = mine + stage * 2 * L::BYTES;
       if (STAGES > 1 && behind == 1) {
         WaitForAllBut<N + (STAGES > 1 ? 1 : 0) * (2 * N + 1)>();
-      } else if (STAGES > 2 && behind == 2) {
-        WaitForAllBut<N + (STAGES > 2 ? 2 : 0) * (2 * N + 1)>();
-      } else if (STAGES > 3 && behind == 3) {
-        WaitForAllBut<N + (STAGES > 3 ? 3 : 0) * (2 * N + 1)>();
       } else {
         WaitForAllBut<N>();
       }
@@ -406,19 +407,11 @@ cached_attention_few_kernel(CachedParams p) {
       if (more) {
         if (STAGES > 1 && behind == 1) {
           WaitForAllBut<N + 1 + (STAGES > 1 ? 1 : 0) * (2 * N + 1)>();
-        } else if (STAGES > 2 && behind == 2) {
-          WaitForAllBut<N + 1 + (STAGES > 2 ? 2 : 0) * (2 * N + 1)>();
-        } else if (STAGES > 3 && behind == 3) {
-          WaitForAllBut<N + 1 + (STAGES > 3 ? 3 : 0) * (2 * N + 1)>();
         } else {
           WaitForAllBut<N + 1>();
         }
       } else if (STAGES > 1 && behind == 1) {
         WaitForAllBut<(STAGES > 1 ? 1 : 0) * (2 * N + 1)>();
-      } else if (STAGES > 2 && behind == 2) {
-        WaitForAllBut<(STAGES > 2 ? 2 : 0) * (2 * N + 1)>();
-      } else if (STAGES > 3 && behind == 3) {
-        WaitForAllBut<(STAGES > 3 ? 3 : 0) * (2 * N + 1)>();
       } else {
         WaitForAllBut<0>();
       }
@@ -494,6 +487,9 @@ cached_attention_few_kernel(CachedParams p) {
 // More pairs, 16-bit types: WQ x 32 pairs, KG wavefronts for each 32 that take the steps of 32 keys in turn, tiles of 64 keys in
 // a ring of four in LDS that loads fill directly, one barrier per tile; the next scores' MFMAs run beside the exponentials.
 // Page numbers come two tiles ahead of the rows; every wavefront places all 64 rows, a lane each, and requests its share.
+// Bound by the matrix cores and the vector unit taking turns: 2.4 us a tile of 64 keys x 192 pairs x 128, whose products alone
+// are 1.3, and the beginning and end of a block's run, 14 us.  8 trees of 48 tokens over 2000 to 5000 bf16 rows, 32 heads over 8 x
+// 128, 64 us; tiles through registers took 113.
 template <typename T, int D, int WQ, int KG>
 __global__ void __launch_bounds__(64 * WQ * KG, 2)
 cached_attention_ring_kernel(CachedParams p) {
@@ -754,7 +750,13 @@ cached_attention_join_kernel(CachedParams p, int keys_per_tile) {
   if (at < p.d) __builtin_memcpy(out, four, sizeof(four));
 }
 
-// Blocks that divide the list of tiles of `keys_per_tile` keys, or one per unit of `runs` x `tile` pairs.
+// Blocks that divide the list of tiles of `keys_per_tile` keys, or one per unit of `runs` x `tile` pairs.  Dividing costs the
+// second kernel, the parts and a beginning more per block, about six tiles, and gains less the more units there are.  us, fp16
+// 12 heads x 64, one token, tiles of 256 keys, divided | not, all sequences of that length (of 64 rows to that length): 1 sequence
+// of 1400 14.0 | 12.7, 2000 13.6 | 15.3, 6000 14.0 | 34.6; 8 of 1400 17.0 | 13.3 (13.9 | 12.7), 2000 20.6 | 15.8 (14.4 | 15.2), 2800
+// 23.1 | 19.7 (14.8 | 19.0), 6000 36.7 | 35.1 (23.3 | 34.7); 16 of 2800 33.1 | 28.2 (17.0 | 18.9), 6000 61.0 | 53.8 (25.4 | 35.4).
+// Tiles of 64 keys, bf16, 48 tokens x 32 heads over 8 x 128: 1 of 250 24.8 | 26.7, 600 27.8 | 41.1, 8 of 250 30.1 | 27.4, 600
+// 32.9 | 42.0.  One block per CU: their wavefronts and buffers leave room for no other.
 template <int D>
 int Divide(CachedParams& p, int tile, int runs, int keys_per_tile, hipStream_t stream) {
   constexpr int kMostBlocks = 256;
@@ -763,7 +765,7 @@ int Divide(CachedParams& p, int tile, int runs, int keys_per_tile, hipStream_t s
   const int units  = p.batch * p.units;
   const int64_t most_tiles = ((int64_t)p.columns * p.page_rows.value + p.tokens + keys_per_tile - 1) / keys_per_tile;
   p.blocks = 0;
-  if (most_tiles > 4) {
+  if (most_tiles > 6 + std::min(units, 192) / 32) {
     const int blocks   = (int)std::min<int64_t>(kMostBlocks, units * most_tiles);
     const size_t bytes = (size_t)2 * blocks * runs * (D * tile / 64 + 2) * 64 * sizeof(float);
     if (bytes <= cinn_hip_kernels::ScratchLimit(cinn_hip_kernels::ScratchKind::kSplitK, stream)) {
@@ -778,7 +780,9 @@ template <typename T, int D, int TILE, int RUNS>
 void LaunchJoin(const CachedParams& p, int keys_per_tile, hipStream_t stream) {
   if (p.blocks == 0) return;
   const int units = p.batch * p.units, wavefronts = units * RUNS * (D * TILE / 256);
-  if (p.blocks / units >= 8) {  // parts of a unit: four a wavefront at a time
+  // parts of a unit, four a wavefront at a time.  The whole call, us, by eight wavefronts | one: one sequence of 100003 fp32 rows 74 |
+  // 85, 30000 33 | 46, one tree of 16 tokens 21.0 | 26.9, of 48 28.9 | 32.0; with eight from two parts on 8 trees of 48 64 | 78
+  if (p.blocks / units >= 8) {
     hipLaunchKernelGGL((cached_attention_join_kernel<T, D, TILE, RUNS, true>), dim3((unsigned)wavefronts), dim3(512), 0, stream, p, keys_per_tile);
   } else {
     hipLaunchKernelGGL((cached_attention_join_kernel<T, D, TILE, RUNS, false>), dim3((unsigned)((wavefronts + 3) / 4)), dim3(256), 0, stream, p,
@@ -807,6 +811,8 @@ void LaunchRing(CachedParams p, hipStream_t stream) {
 
 template <typename T, int D>
 void LaunchTiles(CachedParams p, hipStream_t stream) {
+  // The fewest wavefronts that hold the pairs.  us, bf16 8 sequences of 2000 to 5000 rows, 8 key heads x 128: 32 pairs few 39.7,
+  // ring of 2 x 2 48.5; 64 ring of 2 x 2 45.2, of 4 x 2 45.5; 192 6 x 1 63.3, 8 x 1 63.7; 160 60.7 and 61.0.
   const int pairs = p.tokens * p.group.value;
   if (pairs <= 16) {
     LaunchFew<T, D, 1>(p, stream);

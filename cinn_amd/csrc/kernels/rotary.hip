@@ -7,7 +7,8 @@
 // Bound by memory: every rotated head is read once and written once, out of and into whatever surrounds it.  Angles: p f in
 // turns is a 64-bit product whose fraction is taken before it is rounded to 32 bits (in 32 bits a position of 10^6 would be
 // off by 0.06), then sincospi; a thread keeps those of its pairs for two heads.  Measured: 8191 tokens, 40 of 48 heads x 128
-// in bf16, 168 MB: 27 us, 6.2 TB/s, where a copy of as much moves 5.3; 16 tokens 5.5 us, of which a launch is about 4.
+// in bf16, 168 MB: 34 us out of memory, 4.9 TB/s, where a copy of as much moves 5.3, and 27 us where the last-level cache holds
+// them; 16 tokens 5.5 us, of which a launch is about 4.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
