@@ -33,18 +33,50 @@ struct Found {
   int first, count, tile, more;
 };
 
-// Every wavefront by itself, 64 sequences at a time.  Offsets out of order or range find rows in range all the same.
+// Offsets out of order or range find rows in range all the same.
+struct Sequence {
+  int first, count, tiles;
+};
+__device__ __forceinline__ Sequence SequenceOf(const PackedParams& p, int s, int tile_pairs) {
+  if (s >= p.sequences) return {0, 0, 0};
+  const int first = min(max(p.offsets[s], 0), p.tokens), count = max(min(p.offsets[s + 1], p.tokens) - first, 0);
+  return {first, count, (count * p.group.value + tile_pairs - 1) / tile_pairs};
+}
+
+// The tile of block `tile`, by every wavefront for itself.  Later tiles of a sequence have more keys and come first, of few
+// sequences across all: how many tiles lie at t or further back in their sequences, for 64 values of t at a time, tells the
+// largest t that the block's number falls under.  us, sequence by sequence | across: fp16 12 heads x 64, 8 x 512 rows 17.9 | 15.9,
+// 16 x 512 24.1 | 20.9, 24 x 512 35.5 | 29.3; bf16 32 heads over 8 x 128, 8192 rows in 4 sequences of up to 4000 154 | 154, 16 of
+// up to 1000 42.8 | 43.7, 24 41.8 | 44.4, 64 of up to 250 42.5 | 50.9: the count takes a step for every sequence.
 __device__ __forceinline__ Found Find(const PackedParams& p, int tile, int tile_pairs) {
   const int lane = threadIdx.x & 63;
-  int before     = 0;
-  for (int s0 = 0; s0 < p.sequences; s0 += 64) {
-    int first = 0, count = 0;
-    if (s0 + lane < p.sequences) {
-      first = min(max(p.offsets[s0 + lane], 0), p.tokens);
-      count = max(min(p.offsets[s0 + lane + 1], p.tokens) - first, 0);
+  if (p.sequences <= 16) {
+    const Sequence mine = SequenceOf(p, lane, tile_pairs);
+    int t = 0, after = 0;  // after: how many lie further back than t
+    while (true) {
+      int behind = 0;
+      for (int s = 0; s < p.sequences; s += 4)  // lanes behind the last sequence have none
+#pragma unroll
+        for (int i = 0; i < 4; ++i) behind += max(__builtin_amdgcn_readlane(mine.tiles, s + i) - (t + lane), 0);
+      if (t == 0) {
+        const int all = __builtin_amdgcn_readlane(behind, 0);
+        if (tile >= all) return {0, 0, tile - all, p.tiles - all};
+      }
+      const int last = 63 - __clzll(__ballot(behind > tile));  // lane 0's are more than `tile`
+      t += last;
+      if (last == 63) continue;
+      after = __builtin_amdgcn_readlane(behind, last + 1);
+      break;
     }
-    const int tiles = (count * p.group.value + tile_pairs - 1) / tile_pairs;
-    int sum = tiles;
+    const unsigned long long with = __ballot(mine.tiles > t);
+    const int rank = __popcll(with & ((1ull << lane) - 1));
+    const int at   = __ffsll(__ballot(mine.tiles > t && rank == tile - after)) - 1;
+    return {__builtin_amdgcn_readlane(mine.first, at), __builtin_amdgcn_readlane(mine.count, at), t, 0};
+  }
+  int before = 0;
+  for (int s0 = 0; s0 < p.sequences; s0 += 64) {
+    const Sequence mine = SequenceOf(p, s0 + lane, tile_pairs);
+    int sum = mine.tiles;
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) {
       const int up = __shfl_up(sum, x);
@@ -53,8 +85,8 @@ __device__ __forceinline__ Found Find(const PackedParams& p, int tile, int tile_
     const unsigned long long behind = __ballot(before + sum > tile);
     if (behind) {
       const int at = __ffsll(behind) - 1;
-      const int all = __builtin_amdgcn_readlane(tiles, at), here = tile - (before + __builtin_amdgcn_readlane(sum, at) - all);
-      return {__builtin_amdgcn_readlane(first, at), __builtin_amdgcn_readlane(count, at), all - 1 - here, 0};  // the longest first
+      const int tiles = __builtin_amdgcn_readlane(mine.tiles, at), here = tile - (before + __builtin_amdgcn_readlane(sum, at) - tiles);
+      return {__builtin_amdgcn_readlane(mine.first, at), __builtin_amdgcn_readlane(mine.count, at), tiles - 1 - here, 0};
     }
     before += __builtin_amdgcn_readlane(sum, 63);
   }
@@ -80,7 +112,7 @@ __device__ void ClearRest(const PackedParams& p, int head, int index, int blocks
 // while it takes the exponentials of the last scores: the matrix cores and the vector unit work side by side, within a wavefront
 // and, two of them to a SIMD, across.  Rows behind the last key are rows of the tensor all the same; nothing attends to them.
 // Bound by the matrix cores for long prompts: one of 16384 rows, 32 heads over 8 x 128 in bf16, 1.99 ms, 1.1 PFLOP/s of the 1.25
-// that a product of 8192^3 reaches; 11 prompts of 8191 rows together 203 us; 8 x 512 rows, 12 x 64 in fp16, 18.3 us, a chain of
+// that a product of 8192^3 reaches; 11 prompts of 8191 rows together 203 us; 8 x 512 rows, 12 x 64 in fp16, 16 us, a chain of
 // eight tiles for the last queries.  Tiles that went through registers took 3.2 ms, 334 and 26 us.
 template <typename T, int D, int WQ, int KG, int STEPS>
 __global__ void __launch_bounds__(64 * WQ * KG, 2)
