@@ -66,6 +66,14 @@ def test_many_heads(gpu, kind, lengths, heads, kv_heads, d):
     check(kind, lengths, heads, kv_heads, d, rest=3)
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("lengths,heads", [([1100, 3, 0, 1040], 4), ([1, 2200, 16], 4), ([30, 17] * 8, 6), ([64, 0, 100, 1] * 4 + [65], 2),
+                                           ([0] * 15 + [70], 3), ([5] * 64, 2), ([9] * 65, 1)])
+def test_the_order_of_tiles(gpu, kind, lengths, heads):
+    """sequences of more than 64 tiles, and as many as share one order of their tiles or do not"""
+    check(kind, lengths, heads, 1, 32, lead=2, rest=1)
+
+
 @pytest.mark.parametrize("kind", ["float32", "bfloat16"])
 @pytest.mark.parametrize("lead,rest", [(0, 1), (0, 200), (5, 0), (70, 33)])
 def test_rows_of_no_sequence_are_zero(gpu, kind, lead, rest):
