@@ -540,7 +540,7 @@ cached_attention_ring_kernel(CachedParams p) {
       const unsigned long long word = __ballot(good || (key >= length && key < keys));
       // every wavefront finds and writes the same
       *reinterpret_cast<unsigned long long*>(lds + HOLDS_AT + tile % 8 * 8) = word;
-      if (tile * KT + KT <= length && word != ~0ull) clean = min(clean, tile);
+      if (__ballot(key < length && !good) != 0) clean = min(clean, tile);
       const unsigned to = lds_at + tile % STAGES * STAGE;
       if (even_rows && __ballot(good) == ~0ull) {
 #pragma unroll

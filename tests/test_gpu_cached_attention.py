@@ -171,6 +171,22 @@ def test_pages_that_are_none_hold_no_rows(gpu, kind, tokens):
     case.check()
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("tokens,heads", [(1, 4), (10, 4), (20, 4), (40, 4), (24, 14), (50, 16)])
+@pytest.mark.parametrize("length", [100, 1000, 63, 32])
+def test_the_one_page_that_is_none_lies_where_the_cache_ends(gpu, kind, tokens, heads, length):
+    """the only rows that are none are in the tile that the cache ends in, in its first 32: none of the units' wavefronts (2, 20,
+    40, 80, 168 and 400 pairs of query and head) may count them"""
+    case = Case(kind, [length, length + 64], tokens, heads, 2, 64, 16)
+    for b, end in enumerate((length, length + 64)):
+        case.data["table"][b, end // 64 * 4] = -1
+    # keys whose rows are not there score far below the others, where zeros in their place would weigh most
+    case.data["q"], case.values["q"] = rounded(np.abs(case.values["q"]), kind)
+    for name in ("k", "k_pages"):
+        case.data[name], case.values[name] = rounded(-np.abs(case.values[name]), kind)
+    case.check()
+
+
 @pytest.mark.parametrize("length", [-1, -(1 << 31), (1 << 31) - 1, 161])
 def test_lengths_beyond_the_table(gpu, length):
     case = Case("float16", [160, 100], 3, 4, 2, 32, 16)
