@@ -47,6 +47,14 @@ struct Exp<float> {
   __device__ __forceinline__ float operator()(float s, float base) const { return expf((s - base) * c); }
 };
 
+// Base for probabilities that matrix cores take in T: fp16 ones are held times 2^7, since below 2^-14 its places are 2^-24 for
+// all, and many keys of little weight would be rounded away together.  With maxima that lag by 2^8 at most they stay below
+// 2^15, and are off by 2^-32 of the largest or by half a step, whichever is more.
+template <typename T>
+__device__ __forceinline__ float HeldBase(const Exp<T>& ex, float m) {
+  return __is_same(T, _Float16) ? ex.Base(m) - 7.0f : ex.Base(m);
+}
+
 // a chunk of the query, negated where the scale is negative, zero where it is zero
 template <typename T>
 __device__ __forceinline__ u32x4 Signed(u32x4 v, float scale) {
@@ -205,8 +213,8 @@ struct Queries {
     }
   }
   // The probabilities of 32 keys as the matrix cores take them: 16-bit ones are rounded, which costs half a step of the type
-  // as the result's own rounding does; fp32 operands split in two would take twice the MFMAs.  They are summed before (in twos
-  // by dot products with ones: half the instructions, and 3% slower over 16384 keys).
+  // as the result's own rounding does (fp16 ones far below the largest: HeldBase); fp32 operands split in two would take twice
+  // the MFMAs.  They are summed before (in twos by dot products with ones: half the instructions, and 3% slower over 16384 keys).
   struct Probabilities {
     typename Held<T>::type g[Held<T>::COUNT];
     __device__ __forceinline__ float At(int r) const {  // of register r, which is known after unrolling
@@ -218,7 +226,7 @@ struct Queries {
     }
   };
   __device__ __forceinline__ Probabilities Soften(f32x16 s, const Exp<T>& ex) {
-    const float base = ex.Base(m);
+    const float base = HeldBase(ex, m);
     Probabilities p;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = ex(s[r], base);
@@ -432,7 +440,7 @@ struct FewPairs {
       for (int t = 0; t < DT; ++t) o[tile][t] *= keep;
       m[tile] = top;
     }
-    const float base = ex.Base(m[tile]);
+    const float base = HeldBase(ex, m[tile]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       s[e >> 2][e & 3] = ex(s[e >> 2][e & 3], base);
