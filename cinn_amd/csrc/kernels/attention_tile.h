@@ -96,21 +96,20 @@ struct Shape {
   static constexpr int DT   = (D + 31) / 32;            // 32-row results of O^T
 };
 
-// Rows apart, for tiles that are stored from registers.  K rows are read 16 bytes per lane, rows over lanes: an odd number of
-// 16-byte chunks.  V rows: the four rows of a transposing read, 64 bytes each, fall into different quarters of the banks;
-// single floats: rows four apart do.
-template <typename T, int D>
-struct Padded : Shape<T, D> {
-  using Shape<T, D>::NC, Shape<T, D>::DT, Shape<T, D>::F32;
+// Rows of floats apart, for tiles that are stored from registers.  K rows are read 16 bytes per lane, rows over lanes: an odd
+// number of 16-byte chunks.  V rows, read as single floats: rows four apart fall into different quarters of the banks.
+template <int D>
+struct Padded : Shape<float, D> {
+  using Shape<float, D>::NC, Shape<float, D>::DT, Shape<float, D>::F32;
   static constexpr int K_PITCH = NC * 16 + 16;
-  static constexpr int V_PITCH = F32 ? DT * 128 + 32 : (DT * 64) % 128 == 64 ? DT * 64 : DT * 64 + 64;
+  static constexpr int V_PITCH = DT * 128 + 32;
   static __device__ __forceinline__ int KAt(int row, int c) { return row * K_PITCH + c * 16; }
   static __device__ __forceinline__ int VAt(int row, int c) { return row * V_PITCH + c * 16; }
 };
 
 // Rows behind one another, for tiles that loads write to LDS directly, 64 chunks in order per instruction; the chunks of a row
 // change places instead.  K: eight rows' neighbouring chunks, which LDS serves together, lie in different sixteenths of the
-// banks' 256 bytes.  V: four rows' 64 bytes in different quarters; single floats: the halves for rows four apart.
+// banks' 256 bytes.  V at VAt: four rows' 64 bytes in different quarters.
 template <typename T, int D>
 struct Dense : Shape<T, D> {
   using Shape<T, D>::NC, Shape<T, D>::DT, Shape<T, D>::F32;
@@ -121,10 +120,9 @@ struct Dense : Shape<T, D> {
   static __device__ __forceinline__ int RowTurn(int row) {
     return NC % 16 == 0 ? 2 * (row & 7) : NC % 8 == 0 ? 2 * ((row >> 1) & 3) : 2 * ((row >> 2) & 1);
   }
-  // four rows' 64 bytes, which a transposing read of 32 columns takes together, in different quarters; single floats: the
-  // halves for rows four apart
+  // four rows' 64 bytes, which a transposing read of 32 columns takes together, in different quarters
   static __device__ __forceinline__ int WideTurn(int row) {
-    if (F32) return NC > 8 ? 8 * ((row >> 2) & 1) : 0;
+    static_assert(!F32);
     return NC == 16 ? 4 * (row & 3) : NC == 8 ? 4 * ((row >> 1) & 1) : 0;
   }
   static __device__ __forceinline__ int KTurn(int row) {
@@ -152,7 +150,7 @@ struct Held<float> {
 
 // 32 queries of a wavefront, a lane of either half holding one: S^T = K Q^T leaves the lane 16 scores of its query, register
 // r of key 8 (r / 4) + 4 half + r % 4, and O^T = V^T P^T sixteen sums of each 32 elements of d in the same order.
-template <typename T, int D, class Layout = Padded<T, D>>
+template <typename T, int D, class Layout>
 struct Queries {
   typedef Layout L;
   u32x4 q[L::NC / 2];  // chunks 2 i + half of the query's row

@@ -152,15 +152,17 @@ __device__ __forceinline__ void Finish(const CachedParams& p, Q& rows, int b, in
   }
 }
 
-// D: d rounded up to an instance; WQ x 32 pairs per block, KG groups of wavefronts that take the tiles' keys in turn
-template <typename T, int D, int WQ, int KG>
-__global__ void __launch_bounds__(64 * WQ * KG)
-cached_attention_kernel(CachedParams p) {
-  typedef Queries<T, D> Q;
-  typedef Padded<T, D> L;
-  constexpr int THREADS = 64 * WQ * KG, KT = 32 * KG, NC = L::NC;
+// More than 32 pairs in fp32: 4 x 32 pairs per block, two wavefronts for each 32 that take the tiles' keys in turn, tiles of 64
+// keys through registers into two buffers in LDS.  D: d rounded up to an instance.
+template <int D>
+__global__ void __launch_bounds__(512)
+cached_attention_float_kernel(CachedParams p) {
+  typedef float T;
+  typedef Padded<D> L;
+  typedef Queries<T, D, L> Q;
+  constexpr int WQ = 4, KG = 2, THREADS = 64 * WQ * KG, KT = 32 * KG, NC = L::NC;
   constexpr int V_AT = KT * L::K_PITCH, HOLDS_AT = V_AT + KT * L::V_PITCH, STAGE = HOLDS_AT + KT;
-  constexpr int MEET = (KG - 1) * WQ * 64 * Q::kRegisters * 4;
+  constexpr int MEET = WQ * 64 * Q::kRegisters * 4;
   __shared__ __attribute__((aligned(256))) char lds[2 * STAGE > MEET ? 2 * STAGE : MEET];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave / WQ, wq = wave % WQ;
@@ -235,16 +237,11 @@ cached_attention_kernel(CachedParams p) {
         __syncthreads();
       }
     }
-    if constexpr (KG > 1) {
-      __syncthreads();
-      float* meet = reinterpret_cast<float*>(lds);
-      if (kg > 0) rows.Hand(meet + ((kg - 1) * WQ + wq) * Q::kRegisters * 64, lane);
-      __syncthreads();
-      if (kg == 0) {
-#pragma unroll
-        for (int g = 1; g < KG; ++g) rows.Join(meet + ((g - 1) * WQ + wq) * Q::kRegisters * 64, ex, lane);
-      }
-    }
+    __syncthreads();
+    float* meet = reinterpret_cast<float*>(lds) + wq * Q::kRegisters * 64;
+    if (kg > 0) rows.Hand(meet, lane);
+    __syncthreads();
+    if (kg == 0) rows.Join(meet, ex, lane);
     __syncthreads();  // the next unit's tiles may overwrite what was read here
     if (kg == 0) Finish<T, D>(p, rows, b, head, pair0, lane, tile0 == 0, tile1 == tiles, WQ, wq, seen);
   }
@@ -820,7 +817,7 @@ void LaunchTiles(CachedParams p, hipStream_t stream) {
     LaunchFew<T, D, 2>(p, stream);
   } else if constexpr (sizeof(T) == 4) {
     const int blocks = Divide<D>(p, 32, 4, 64, stream);
-    hipLaunchKernelGGL((cached_attention_kernel<T, D, 4, 2>), dim3((unsigned)blocks), dim3(512), 0, stream, p);
+    hipLaunchKernelGGL((cached_attention_float_kernel<D>), dim3((unsigned)blocks), dim3(512), 0, stream, p);
     LaunchJoin<T, D, 32, 4>(p, 64, stream);
   } else if (pairs <= 64) {
     LaunchRing<T, D, 2, 2>(p, stream);

@@ -261,18 +261,18 @@ packed_attention_ring_kernel(PackedParams p) {
   rows.Store(out, p.d, 1.0f / sum, half);
 }
 
-// The same with 16 x PT pairs a wavefront, for few pairs and for fp32: shorter chains of MFMAs and exponentials per step, and
+// The same with 16 pairs a wavefront, for few pairs and for fp32: shorter chains of MFMAs and exponentials per step, and
 // twice the wavefronts, where latency counts.  Bound by a wavefront's own instructions, one after the other: 5 prompts of 17 to
 // 100 rows, 8 heads over 2 x 80 in fp32, 16.6 us.
-template <typename T, int D, int PT, int WAVES>
+template <typename T, int D, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, 2)
 packed_attention_few_kernel(PackedParams p) {
-  typedef FewPairs<T, D, PT> Q;
+  typedef FewPairs<T, D, 1> Q;
   typedef Dense<T, D> L;
   constexpr int NC = L::NC, STAGE = 2 * L::BYTES, STAGES = 4, LOADS = NC, N = (LOADS + WAVES - 1) / WAVES;  // the last is asked for again
   __shared__ __attribute__((aligned(256))) char lds[STAGES * STAGE];
   const int head = blockIdx.x % p.kv_heads;
-  const Found at = Find(p, blockIdx.x / p.kv_heads, 16 * PT * WAVES);
+  const Found at = Find(p, blockIdx.x / p.kv_heads, 16 * WAVES);
   if (at.count == 0) {
     ClearRest<T>(p, head, at.tile, at.more);
     return;
@@ -280,10 +280,10 @@ packed_attention_few_kernel(PackedParams p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int chunks = p.d * (int)sizeof(T) / 16, group = p.group.value, pairs = at.count * group;
-  const int pair0 = (at.tile * WAVES + wave) * 16 * PT;
+  const int pair0 = (at.tile * WAVES + wave) * 16;
   const int first_query = p.group(min(pair0, pairs - 1));
-  const int last_query  = pair0 < pairs ? p.group(min(pair0 + 16 * PT - 1, pairs - 1)) : -1;
-  const int keys  = p.group(min((at.tile + 1) * WAVES * 16 * PT, pairs) - 1) + 1;
+  const int last_query  = pair0 < pairs ? p.group(min(pair0 + 15, pairs - 1)) : -1;
+  const int keys  = p.group(min((at.tile + 1) * WAVES * 16, pairs) - 1) + 1;
   const int steps = (keys + 31) / 32, my_steps = __builtin_amdgcn_readfirstlane(last_query >= 0 ? last_query / 32 + 1 : 0);
   const int plain_steps = __builtin_amdgcn_readfirstlane(last_query >= 0 ? (first_query + 1) / 32 : 0);
 
@@ -322,14 +322,8 @@ packed_attention_few_kernel(PackedParams p) {
 #pragma unroll 1
   for (int i = 0; i < STAGES - 1 && i < steps; ++i) request(i);
   Q rows;
-  int query[PT];
-#pragma unroll
-  for (int n = 0; n < PT; ++n) {
-    const int pair = min(pair0 + n * 16 + (lane & 15), pairs - 1);
-    query[n] = p.group(pair);
-    rows.Start(n, HeadOf<T>(p.q, 0, head * group + pair - query[n] * group) + (at.first + query[n]) * p.q.row * (int64_t)sizeof(T), chunks, lane,
-               p.scale);
-  }
+  const int pair = min(pair0 + (lane & 15), pairs - 1), query = p.group(pair), my_head = head * group + pair - query * group;
+  rows.Start(0, HeadOf<T>(p.q, 0, my_head) + (at.first + query) * p.q.row * (int64_t)sizeof(T), chunks, lane, p.scale);
   const Exp<T> ex(p.scale);
   WaitForAllBut<0>();  // the queries are the last that was asked for
   __builtin_amdgcn_s_barrier();
@@ -346,17 +340,14 @@ packed_attention_few_kernel(PackedParams p) {
     asm volatile("" ::: "memory");
     if (step + STAGES - 2 < steps) request(step + STAGES - 2);
   };
-  f32x4 s[PT][2];
-  unsigned word[PT];
+  f32x4 s[1][2];
+  unsigned word[1];
   auto keys_of   = [&](int n) { return lds + n % STAGES * STAGE; };
   auto values_of = [&](int n) { return keys_of(n) + L::BYTES; };
   int step = 0;
   auto open = [&] {  // the step's scores are complete
-#pragma unroll
-    for (int n = 0; n < PT; ++n) {
-      word[n] = Below(query[n] + 1 - step * 32);
-      if (step >= plain_steps) Q::Mask(s[n], word[n], lane);
-    }
+    word[0] = Below(query + 1 - step * 32);
+    if (step >= plain_steps) Q::Mask(s[0], word[0], lane);
   };
   rows.Scores(s, keys_of(0), lane);
 #pragma unroll 1
@@ -365,12 +356,8 @@ packed_attention_few_kernel(PackedParams p) {
     turn(step + 1);
     if (step >= my_steps) continue;
     if (step >= plain_steps && Q::Unbounded(values_of(step), lane)) break;
-    f32x4 mine[PT][2];
-#pragma unroll
-    for (int n = 0; n < PT; ++n) {
-      rows.Soften(n, s[n], ex);
-      mine[n][0] = s[n][0], mine[n][1] = s[n][1];
-    }
+    rows.Soften(0, s[0], ex);
+    const f32x4 mine[1][2] = {{s[0][0], s[0][1]}};
     rows.Scores(s, keys_of(step + 1), lane);
     rows.Add(mine, values_of(step), lane);
   }
@@ -382,20 +369,14 @@ packed_attention_few_kernel(PackedParams p) {
       turn(step + 1);
     }
     if (step >= my_steps) continue;
-#pragma unroll
-    for (int n = 0; n < PT; ++n) rows.Soften(n, s[n], ex);
+    rows.Soften(0, s[0], ex);
     rows.AddChosen(s, word, values_of(step), lane);
     rows.Scores(s, keys_of(step + 1), lane);
   }
-#pragma unroll
-  for (int n = 0; n < PT; ++n) {
-    float sum = rows.l[n] + __shfl_xor(rows.l[n], 16);
-    sum += __shfl_xor(sum, 32);
-    const int pair = pair0 + n * 16 + (lane & 15);
-    if (pair >= pairs) continue;
-    rows.Store(n, const_cast<char*>(HeadOf<T>(p.o, 0, head * group + pair - query[n] * group)) + (at.first + query[n]) * p.o.row * (int64_t)sizeof(T),
-               p.d, 1.0f / sum, lane);
-  }
+  float sum = rows.l[0] + __shfl_xor(rows.l[0], 16);
+  sum += __shfl_xor(sum, 32);
+  if (pair0 + (lane & 15) >= pairs) return;
+  rows.Store(0, const_cast<char*>(HeadOf<T>(p.o, 0, my_head)) + (at.first + query) * p.o.row * (int64_t)sizeof(T), p.d, 1.0f / sum, lane);
 }
 
 template <typename T, int D, int WQ, int KG, int STEPS>
@@ -418,7 +399,7 @@ void LaunchTiles(PackedParams p, hipStream_t stream) {
   }
   constexpr int kPairs = 64;
   p.tiles = (int)((int64_t)p.tokens * p.group.value / kPairs) + p.sequences + 1;
-  hipLaunchKernelGGL((packed_attention_few_kernel<T, D, 1, kPairs / 16>), dim3((unsigned)p.tiles * p.kv_heads), dim3(kPairs * 4), 0, stream, p);
+  hipLaunchKernelGGL((packed_attention_few_kernel<T, D, kPairs / 16>), dim3((unsigned)p.tiles * p.kv_heads), dim3(kPairs * 4), 0, stream, p);
 }
 
 template <typename T>
