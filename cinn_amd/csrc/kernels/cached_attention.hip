@@ -153,7 +153,8 @@ __device__ __forceinline__ void Finish(const CachedParams& p, Q& rows, int b, in
 }
 
 // More than 32 pairs in fp32: 4 x 32 pairs per block, two wavefronts for each 32 that take the tiles' keys in turn, tiles of 64
-// keys through registers into two buffers in LDS.  D: d rounded up to an instance.
+// keys through registers into two buffers in LDS.  D: d rounded up to an instance.  8 trees of 48 tokens over 2000 to 5000 rows, 32 heads
+// over 8 x 128, 410 us; the products alone would take 144.
 template <int D>
 __global__ void __launch_bounds__(512)
 cached_attention_float_kernel(CachedParams p) {
@@ -484,9 +485,9 @@ cached_attention_few_kernel(CachedParams p) {
 // More pairs, 16-bit types: WQ x 32 pairs, KG wavefronts for each 32 that take the steps of 32 keys in turn, tiles of 64 keys in
 // a ring of four in LDS that loads fill directly, one barrier per tile; the next scores' MFMAs run beside the exponentials.
 // Page numbers come two tiles ahead of the rows; every wavefront places all 64 rows, a lane each, and requests its share.
-// Bound by the matrix cores and the vector unit taking turns: 2.4 us a tile of 64 keys x 192 pairs x 128, whose products alone
-// are 1.3, and the beginning and end of a block's run, 14 us.  8 trees of 48 tokens over 2000 to 5000 bf16 rows, 32 heads over 8 x
-// 128, 64 us; tiles through registers took 113.
+// 2.4 us a tile of 64 keys x 192 pairs x 128, whose products alone are 0.9 where a vector unit has two of the six wavefronts, and the
+// beginning and end of a block's run, 14 us; wavefronts wait in half of their cycles, matrix cores are busy in 18% and vector units
+// in 29%.  8 trees of 48 tokens over 2000 to 5000 bf16 rows, 32 heads over 8 x 128, 62 us; tiles through registers took 113.
 template <typename T, int D, int WQ, int KG>
 __global__ void __launch_bounds__(64 * WQ * KG, 2)
 cached_attention_ring_kernel(CachedParams p) {
@@ -754,6 +755,8 @@ cached_attention_join_kernel(CachedParams p, int keys_per_tile) {
 // 23.1 | 19.7 (14.8 | 19.0), 6000 36.7 | 35.1 (23.3 | 34.7); 16 of 2800 33.1 | 28.2 (17.0 | 18.9), 6000 61.0 | 53.8 (25.4 | 35.4).
 // Tiles of 64 keys, bf16, 48 tokens x 32 heads over 8 x 128: 1 of 250 24.8 | 26.7, 600 27.8 | 41.1, 8 of 250 30.1 | 27.4, 600
 // 32.9 | 42.0.  One block per CU: their wavefronts and buffers leave room for no other.
+// The lengths are the GPU's, so the table's width stands for them, and short caches in wide tables pay for being divided: 8 of 511
+// rows 7.2 in tables for up to 2048 rows, 13.0 for 8192 and 131072; 1 of 511 7.0 and 11.5; 8 of 2000 15.5 and 20.2.
 template <int D>
 int Divide(CachedParams& p, int tile, int runs, int keys_per_tile, hipStream_t stream) {
   constexpr int kMostBlocks = 256;
@@ -809,7 +812,8 @@ void LaunchRing(CachedParams p, hipStream_t stream) {
 template <typename T, int D>
 void LaunchTiles(CachedParams p, hipStream_t stream) {
   // The fewest wavefronts that hold the pairs.  us, bf16 8 sequences of 2000 to 5000 rows, 8 key heads x 128: 32 pairs few 39.7,
-  // ring of 2 x 2 48.5; 64 ring of 2 x 2 45.2, of 4 x 2 45.5; 192 6 x 1 63.3, 8 x 1 63.7; 160 60.7 and 61.0.
+  // ring of 2 x 2 48.5.  The choices among rings are worth 1% or nothing, the smaller | the larger in turn: 2 x 2 | 4 x 2 with 36, 48,
+  // 64 pairs 45.0 | 45.0, 44.5 | 44.4, 44.7 | 44.6; 6 x 1 | 8 x 1 with 144, 160, 192 pairs 60.1 | 60.4, 60.2 | 60.6, 61.9 | 62.3.
   const int pairs = p.tokens * p.group.value;
   if (pairs <= 16) {
     LaunchFew<T, D, 1>(p, stream);

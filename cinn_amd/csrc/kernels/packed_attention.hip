@@ -111,9 +111,10 @@ __device__ void ClearRest(const PackedParams& p, int head, int index, int blocks
 // ring of four in LDS that loads fill directly, one barrier per tile.  A wavefront multiplies the next 32 keys by its queries
 // while it takes the exponentials of the last scores: the matrix cores and the vector unit work side by side, within a wavefront
 // and, two of them to a SIMD, across.  Rows behind the last key are rows of the tensor all the same; nothing attends to them.
-// Bound by the matrix cores for long prompts: one of 16384 rows, 32 heads over 8 x 128 in bf16, 1.99 ms, 1.1 PFLOP/s of the 1.25
-// that a product of 8192^3 reaches; 11 prompts of 8191 rows together 203 us; 8 x 512 rows, 12 x 64 in fp16, 16 us, a chain of
-// eight tiles for the last queries.  Tiles that went through registers took 3.2 ms, 334 and 26 us.
+// Bound by matrix cores and vector units together for long prompts, 53 and 50 % of whose cycles are taken: one of 16384 rows, 32 heads
+// over 8 x 128 in bf16, 2.00 to 2.06 ms, 1.1 PFLOP/s of the 1.25 that a product of 8192^3 reaches; 11 prompts of 8191 rows together
+// 201 to 208 us; 8 x 512 rows, 12 x 64 in fp16, 15.7 us, a chain of eight tiles for the last queries, wavefronts waiting in 56 % of
+// their cycles.  Tiles that went through registers took 3.2 ms, 334 and 26 us.
 template <typename T, int D, int WQ, int KG, int STEPS>
 __global__ void __launch_bounds__(64 * WQ * KG, 2)
 packed_attention_ring_kernel(PackedParams p) {
@@ -262,8 +263,9 @@ packed_attention_ring_kernel(PackedParams p) {
 }
 
 // The same with 16 pairs a wavefront, for few pairs and for fp32: shorter chains of MFMAs and exponentials per step, and
-// twice the wavefronts, where latency counts.  Bound by a wavefront's own instructions, one after the other: 5 prompts of 17 to
-// 100 rows, 8 heads over 2 x 80 in fp32, 16.6 us.
+// twice the wavefronts, where latency counts.  5 prompts of 17 to 100 rows, 8 heads over 2 x 80 in fp32, 16.7 us on 40 blocks, bound by
+// a wavefront's latencies with nothing beside it: 44% of its cycles wait for memory, LDS and barriers, 23% for instructions that
+// may not issue yet, 33% issue.
 template <typename T, int D, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, 2)
 packed_attention_few_kernel(PackedParams p) {
@@ -389,9 +391,12 @@ template <typename T, int D>
 void LaunchTiles(PackedParams p, hipStream_t stream) {
   // Blocks of 128 pairs: how full the GPU is, whatever the lengths.  us, few | ring of 4 x 2 | 4 x 1 | 8 x 1 wavefronts, the
   // choice in brackets.  bf16 32 heads over 8 x 128, one prompt of 64 [7.2] | 10.2 | 9.1 | 10.7, 256 [11.7] | 13.5 | 13.7 |
-  // 16.2, 1024 31.9 | [28.4] | 34.0 | 39.6, 2048 74.7 | [59.4] | 64.1 | 70.9, 4096 - | - | 150 | [142], 16384 - | - | 2100 |
-  // [1995]; 11 ragged prompts of 8126 330 | 264 | 205 | [200].  The wavefronts of a block wait for the one with the last
-  // queries: with one head a key head 256 queries apart, fp16 12 heads x 64, 8 x 1024 - | - | [33] | 37.
+  // 16.2, 1024 31.9 | [28.4] | 34.0 | 39.6, 2048 74.7 | [59.4] | 64.1 | 70.9, 4096 - | - | 152 | [144], 16384 - | - | 2100 |
+  // [1995]; 11 ragged prompts of 8191 330 | 264 | 201 | [201].  The wavefronts of a block wait for the one with the last
+  // queries, with one head a key head 256 queries apart, which costs where prompts are not long.  4 x 1 | 8 x 1 by heads a key
+  // head, 1, 2, 3, 4, 8: fp16 12 heads x 64, 8 x 1024 32.6 | 34.5, 30.5 | 31.6, 29.9 | 30.7, 29.7 | 30.4, -; 8 x 2048 83 | 81, 81 | 76,
+  // 81 | 75, 81 | 76, -; bf16 32 or 33 x 128, one of 4096 159 | 151, 152 | 146, 160 | 161, 152 | 144, 153 | 146, ragged 215 | 222, 201 |
+  // 202, 227 | 216, 201 | 201, 202 | 200: within 8% of each other, the lengths, which the host does not know, counting as much.
   const int64_t blocks = (int64_t)p.tokens * p.group.value / 128 * p.kv_heads;
   if constexpr (sizeof(T) == 2) {
     if (blocks > 512) return p.group.value >= 4 ? LaunchRing<T, D, 8, 1, 2>(p, stream) : LaunchRing<T, D, 4, 1, 1>(p, stream);

@@ -8,7 +8,7 @@
 // turns is a 64-bit product whose fraction is taken before it is rounded to 32 bits (in 32 bits a position of 10^6 would be
 // off by 0.06), then sincospi; a thread keeps those of its pairs for two heads.  Measured: 8191 tokens, 40 of 48 heads x 128
 // in bf16, 168 MB: 34 us out of memory, 4.9 TB/s, where a copy of as much moves 5.3, and 27 us where the last-level cache holds
-// them; 16 tokens 5.5 us, of which a launch is about 4.
+// them; 16 tokens 4.7 to 5.6 us, of which a launch is about 4.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -125,8 +125,9 @@ template <typename T, int V>
 void Launch(RotaryParams p, const Turns& turns, int64_t tokens, bool neighbours, hipStream_t stream) {
   p.pair_units = neighbours ? 2 * p.pairs / V : p.pairs / V;
   p.units      = p.pair_units + (p.d - 2 * p.pairs + V - 1) / V;
-  // us with 1 | 2 | 4 | 8 heads a thread: 8191 tokens x 40 heads x 128 in bf16 33.5 | 27.3 | 28.0 | 28.4, 512 tokens 6.1 | 5.3 |
-  // 5.2 | 6.2, 16 tokens 5.7 | 5.5 | 5.3 | 6.0, 1111 x 12 x 80 in fp32 5.1 | 4.8 | 5.1 | 5.7
+  // us with 1 | 2 | 4 | 8 heads a thread: 8191 tokens x 40 heads x 128 in bf16 out of memory 40.1 | 34.9 | 36.4 | 36.6, out of the
+  // last-level cache 33.6 | 27.5 | 28.1 | 28.9; 16384 x 40 x 64 in fp16 out of memory 39.6 | 34.9 | 36.7 | 38.7; 512 tokens 5.5 | 5.4 |
+  // 5.3 | 6.2, 16 tokens 5.1 | 5.5 | 5.6 | 5.6, 1111 x 12 x 80 in fp32 4.8 | 5.1 | 5.2 | 5.7
   p.heads_each  = 2;
   p.head_groups = (p.heads + p.heads_each - 1) / p.heads_each;
   p.threads     = tokens * p.head_groups * p.units;
